@@ -39,7 +39,8 @@ typedef enum {
     TERNOCL_ERR_WORKSPACE = 7   /* workspace too small */
 } ternocl_status;
 
-typedef enum { TERNOCL_FP16 = 0, TERNOCL_BF16 = 1 } ternocl_dtype;
+/* TERNOCL_FP32 is a type of ternocl_moe_topk's logits and weights only. */
+typedef enum { TERNOCL_FP16 = 0, TERNOCL_BF16 = 1, TERNOCL_FP32 = 2 } ternocl_dtype;
 
 /* Fused epilogue, applied to the fp32 accumulator before the output cast
  * (common/epilogue.clh:1-37). */
@@ -69,8 +70,8 @@ const char *ternocl_status_string(int status);
 const char *ternocl_last_error(void);
 /* Device-side error word of the current device (synchronous read): bit 0 = a bounded
  * wait inside a kernel gave up (the kernel returned without hanging; its outputs are
- * invalid); bit 1 = ternocl_moe_route met an expert id outside [0, E) (that row was
- * left out).  reset != 0 clears it.  Returns -1 if it cannot be read. */
+ * invalid); bit 1 = ternocl_moe_route or an MoE decode call met an expert id outside
+ * [0, E) (that row was left out).  reset != 0 clears it.  Returns -1 if it cannot be read. */
 int ternocl_device_error(int reset);
 
 /* Process-wide options.
@@ -342,6 +343,66 @@ int ternocl_moe_decode_down_sum(const int32_t *ids, const void *H, const void *R
                                 void *stream);
 
 /* ---------------------------------------------------------------------------------
+ * 4-bit weights with group scales (no counterpart in the reference): for the layers of a
+ * ternary model that keep more bits (output head, first layers, sensitive experts).
+ *   weight(k, n) = code(k, n) * S[k/128, n],   code in -8..7
+ *   B : uint32 [K/8, N], code of row 8kp+j at bits 4j..4j+3 (two's complement)
+ *   S : DT [K/128, N]
+ * The other tensors, the epilogues and the N % 16 / K % 128 rules are ternocl_int2_upcvt's.
+ * Codes and activations are multiplied exactly and each 128-row group's fp32 sum is scaled
+ * by S: no dequantised weight is rounded, at any M.  A row of A with an Inf or a NaN gives
+ * values that are not finite or not meaningful in that row of C only.
+ *
+ * Linear layer:  C[m,n] = DT(epi( sum_k A[m,k] * code(B[k,n]) * S[k/128, n] )).
+ * algo: GEMV (decode), GEMM (tcgen05), or AUTO (the GEMV up to M = 8).  No workspace: a K
+ * split stays within one thread-block cluster.  M <= 524280. */
+int ternocl_int4_upcvt(const void *A, const uint32_t *B, const void *S, void *C, const void *Other,
+                       const void *Bias, int M, int N, int K, int dtype, int postop, int out_f32, int algo,
+                       void *stream);
+
+/* Grouped GEMM of MoE prefill with 4-bit experts, as ternocl_moe_gemm: for the rows p of
+ * every expert e (meta of ternocl_moe_route), C[p, n] = epi(A[p] . B_e[:, n]); B_all
+ * [E, K/8, N], S_all [E, K/128, N]; Other_all [G, N] (POSTOP 1/2); no bias.  Rows of C that
+ * belong to no expert are not written.  G <= 2^20. */
+int ternocl_moe_gemm_int4(const int32_t *meta, const void *A_all, const uint32_t *B_all, const void *S_all,
+                          void *C_all, const void *Other_all, int G, int N, int K, int num_experts, int dtype,
+                          int postop, int out_f32, void *stream);
+
+/* MoE decode with 4-bit experts, as ternocl_moe_decode_gate_up and _down_sum: every routed
+ * (token, expert) pair in one launch; B* [E, K/8, N], S* [E, K/128, N].  An expert id outside
+ * [0, E) contributes zero and sets bit 1 of ternocl_device_error.
+ *   gate_up:   H[g, n] = DT(silu(X[g/topk] . gate_e[:, n]) * (X[g/topk] . up_e[:, n]))
+ *   down_sum:  O[t, n] = DT(sum_j RW[g] * (H[g] . down_e[:, n])),  g = t*topk + j, e = ids[g] */
+int ternocl_moe_decode_gate_up_int4(const int32_t *ids, const void *X, const uint32_t *Bg, const void *Sg,
+                                    const uint32_t *Bu, const void *Su, void *H, int G, int N, int K, int topk,
+                                    int num_experts, int dtype, void *stream);
+int ternocl_moe_decode_down_sum_int4(const int32_t *ids, const void *H, const void *RW, const uint32_t *B,
+                                     const void *S, void *O, int T, int N, int K, int topk, int num_experts,
+                                     int dtype, void *stream);
+
+/* ---------------------------------------------------------------------------------
+ * The experts' choice from router logits (no counterpart in the reference, whose drivers
+ * generate ids and weights): makes the ids of ternocl_moe_route / _moe_decode_* and the RW of
+ * ternocl_moe_combine / _moe_decode_down*.
+ *   s = softmax(logits[t]) or sigmoid(logits[t])      c = s + bias  (bias [E] fp32, or NULL)
+ *   the E experts form n_group groups of neighbours; a group's score is the sum of its
+ *   group_top (1 or 2) largest c; the topk_group best groups are kept (n_group = 1: all)
+ *   ids[t, :] = the topk experts of the kept groups with the largest c, descending
+ *   RW[t, j]  = s[ids[t, j]], / (sum over j) if renormalize, * scale
+ * Ties go to the lowest index.  Without a bias the order is that of the logits; with one,
+ * and for the groups' scores, c is computed in 64 bits.  An expert whose logit or bias is NaN or -inf is
+ * masked: left out of the softmax, chosen after every other expert of the kept groups
+ * (lowest index first), weight 0; a group with fewer than group_top unmasked experts comes
+ * after the others.  A logit of +inf counts as the largest finite fp32.  Where the sum is 0 the
+ * weights are 0.  So ids always holds topk distinct experts of [0, E).
+ * logits [T, E] and RW [T, topk] in their own types (fp16, bf16 or fp32).  E <= 1024,
+ * topk <= 32 and <= topk_group * E / n_group, n_group <= 32 dividing E. */
+typedef enum { TERNOCL_SCORE_SOFTMAX = 0, TERNOCL_SCORE_SIGMOID = 1 } ternocl_score;
+int ternocl_moe_topk(const void *logits, const float *bias, int32_t *ids, void *RW, int T, int E, int topk,
+                     int scoring, int n_group, int topk_group, int group_top, int renormalize, float scale,
+                     int logits_dtype, int rw_dtype, void *stream);
+
+/* ---------------------------------------------------------------------------------
  * Host-side weight packers (no device work).  Same layouts as the reference's
  * common/bitcos.hpp and int1 driver.
  *
@@ -353,6 +414,9 @@ size_t ternocl_bitcos_random(int K, int N, double z, uint64_t seed, uint32_t *ou
 size_t ternocl_bitcos_pack(const int8_t *codes, int K, int N, uint32_t *out, size_t cap);
 /* slice_ranks [(ls-1), N] (common/bitcos.hpp:81-94). */
 int ternocl_bitcos_slice_ranks(const uint32_t *buf, int K, int N, int ls, uint32_t *out);
+/* Pack codes [K, N] (row-major, values -8..7) into the 4-bit layout [K/8, N]; ERR_ARG for a
+ * code outside that range. */
+int ternocl_int4_pack(const int8_t *codes, int K, int N, uint32_t *out);
 /* int1 per-column bit order [K/32, N] -> device sel layout (int1_fp16_upcvt/main.cpp:80-92). */
 int ternocl_int1_to_sel(const uint32_t *B, uint32_t *out, int K, int N);
 

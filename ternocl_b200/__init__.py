@@ -9,9 +9,10 @@ keyword arguments.  Errors raise TernoclError; there is no CPU fallback.
 """
 from ._lib import LIB_PATH, TernoclError, call, header_functions, lib  # noqa: F401
 
-FP16, BF16 = 0, 1
+FP16, BF16, FP32 = 0, 1, 2  # FP32: moe_topk only
 POSTOP_NONE, POSTOP_SILU_MUL, POSTOP_ADD, POSTOP_BIAS, POSTOP_SIGMOID = range(5)
 ALGO_AUTO, ALGO_GEMV, ALGO_GEMM, ALGO_GEMV_TMEM = 0, 1, 2, 3
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 OPT_PDL = 1
 OPT_GEMM_TILE_M = 2
 OPT_GEMV_SPLIT = 3
@@ -365,3 +366,165 @@ def moe_decode_down_sum(ids, H, RW, B, S, num_experts, topk, out=None, stream=No
     call("ternocl_moe_decode_down_sum", _ptr(ids), _ptr(H), _ptr(RW), _ptr(B), _ptr(S), _ptr(O), T, N, K, int(topk),
          int(num_experts), dtype_code(H), _stream(stream))
     return O
+
+
+# ---- 4-bit weights and the experts' choice ------------------------------------------------
+def _launch(name, like, stream, *args):
+    """Call entry point `name` on `like`'s device (made current for the call if it is not); no rows, no call."""
+    torch = _torch()
+    if like.shape[0] == 0:
+        return None
+    if like.device.index == torch.cuda.current_device():
+        return call(name, *args, _stream(stream))
+    with torch.cuda.device(like.device):
+        return call(name, *args, _stream(stream))
+
+
+def _expect(name, t, shape, dtype, like):
+    """`t` is a contiguous CUDA tensor of this shape and dtype on `like`'s device."""
+    if not t.is_cuda or not t.is_contiguous() or t.device != like.device:
+        raise ValueError("%s must be a contiguous CUDA tensor on %s" % (name, like.device))
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
+    if t.dtype != dtype:
+        raise TypeError("%s must be %s, got %s" % (name, dtype, t.dtype))
+
+
+def _expect_int4(name, B, S, lead, K, N, like):
+    torch = _torch()
+    if K % 128 or N % 16:
+        raise ValueError("%s: K %% 128 == 0 and N %% 16 == 0 needed, got K = %d, N = %d" % (name, K, N))
+    _expect(name, B, (*lead, K // 8, N), torch.int32, like)
+    _expect("the scales of " + name, S, (*lead, K // 128, N), like.dtype, like)
+
+
+def _rows2(name, A):
+    if A.dim() != 2:
+        raise ValueError("%s must be [rows, K], got %s" % (name, tuple(A.shape)))
+    _expect(name, A, A.shape, A.dtype, A)
+    return dtype_code(A), A.shape[0], A.shape[1]
+
+
+def _result(out, shape, dtype, like):
+    if out is None:
+        return _torch().empty(shape, dtype=dtype, device=like.device)
+    _expect("out", out, shape, dtype, like)
+    return out
+
+
+def _int4_epilogue(A, M, N, postop, out_f32, other, bias):
+    torch = _torch()
+    if postop in (POSTOP_SILU_MUL, POSTOP_ADD):
+        if other is None:
+            raise ValueError("postop %d needs other" % postop)
+        _expect("other", other, (M, N), A.dtype, A)
+    if postop == POSTOP_BIAS:
+        if bias is None:
+            raise ValueError("postop 3 needs bias")
+        _expect("bias", bias, (N,), torch.float32 if out_f32 else A.dtype, A)
+    return torch.float32 if out_f32 else A.dtype
+
+
+def int4_upcvt(A, B, S, postop=0, out_f32=False, other=None, bias=None, out=None, algo=0, stream=None):
+    """C = epi(A @ dequant_int4(B, S)); A [M,K] fp16/bf16, B int32 [K/8,N] (row 8i+j at bits 4j, codes -8..7),
+    S [K/128,N].  Codes and activations are multiplied exactly; scales are applied to fp32 group sums."""
+    dt, M, K = _rows2("A", A)
+    N = B.shape[-1]
+    _expect_int4("B", B, S, (), K, N, A)
+    C = _result(out, (M, N), _int4_epilogue(A, M, N, postop, out_f32, other, bias), A)
+    _launch("ternocl_int4_upcvt", A, stream, _ptr(A), _ptr(B), _ptr(S), _ptr(C), _ptr(other), _ptr(bias), M, N, K, dt,
+            int(postop), int(bool(out_f32)), int(algo))
+    return C
+
+
+def int4_pack(codes):
+    """codes [K, N] in -8..7 -> host int4 weights (numpy uint32 [K/8, N])."""
+    import numpy as np
+    codes = np.asarray(codes)
+    if codes.size and (codes.min() < -8 or codes.max() > 7):
+        raise ValueError("codes must lie in -8..7")
+    codes = np.ascontiguousarray(codes, np.int8)
+    K, N = codes.shape
+    out = np.empty((K // 8, N), np.uint32)
+    call("ternocl_int4_pack", codes.ctypes.data, K, N, out.ctypes.data)
+    return out
+
+
+def moe_gemm_int4(meta, A, B_all, S_all, num_experts, postop=0, out_f32=False, other=None, out=None, stream=None):
+    """Per-expert C[p] = epi(A[p] @ dequant_int4(B_all[e], S_all[e])) for the sorted rows p of expert e.
+    A [G, K]; B_all int32 [E, K/8, N]; S_all [E, K/128, N]; other [G, N] for POSTOP 1/2."""
+    torch = _torch()
+    dt, G, K = _rows2("A", A)
+    N, E = B_all.shape[-1], int(num_experts)
+    _expect_int4("B_all", B_all, S_all, (E,), K, N, A)
+    _expect("meta", meta, (2 * E + 2,), torch.int32, A)
+    C = _result(out, (G, N), _int4_epilogue(A, G, N, postop, out_f32, other, None) if postop != POSTOP_BIAS else A.dtype,
+                A)
+    _launch("ternocl_moe_gemm_int4", A, stream, _ptr(meta), _ptr(A), _ptr(B_all), _ptr(S_all), _ptr(C), _ptr(other), G,
+            N, K, E, dt, int(postop), int(bool(out_f32)))
+    return C
+
+
+def moe_decode_gate_up_int4(ids, X, Bg, Sg, Bu, Su, num_experts, topk, out=None, stream=None):
+    """H[g] = silu(X[g/topk] . gate_e) * (X[g/topk] . up_e), e = ids[g]; Bg/Bu int32 [E, K/8, N]."""
+    torch = _torch()
+    dt, T, K = _rows2("X", X)
+    N, E, topk = Bg.shape[-1], int(num_experts), int(topk)
+    G = T * topk
+    _expect("ids", ids, (G,), torch.int32, X)
+    _expect_int4("Bg", Bg, Sg, (E,), K, N, X)
+    _expect_int4("Bu", Bu, Su, (E,), K, N, X)
+    H = _result(out, (G, N), X.dtype, X)
+    _launch("ternocl_moe_decode_gate_up_int4", X, stream, _ptr(ids), _ptr(X), _ptr(Bg), _ptr(Sg), _ptr(Bu), _ptr(Su),
+            _ptr(H), G, N, K, topk, E, dt)
+    return H
+
+
+def moe_decode_down_sum_int4(ids, H, RW, B, S, num_experts, topk, out=None, stream=None):
+    """O[t] = sum_j RW[g] * (H[g] . down_e), g = t*topk + j, e = ids[g]; B int32 [E, K/8, N]."""
+    torch = _torch()
+    dt, G, K = _rows2("H", H)
+    N, E, topk = B.shape[-1], int(num_experts), int(topk)
+    if topk < 1 or G % topk:
+        raise ValueError("H must have topk rows for each token, got %d rows, topk = %d" % (G, topk))
+    T = G // topk
+    _expect("ids", ids, (G,), torch.int32, H)
+    _expect("RW", RW, (G,), H.dtype, H)
+    _expect_int4("B", B, S, (E,), K, N, H)
+    O = _result(out, (T, N), H.dtype, H)
+    _launch("ternocl_moe_decode_down_sum_int4", H, stream, _ptr(ids), _ptr(H), _ptr(RW), _ptr(B), _ptr(S), _ptr(O), T,
+            N, K, topk, E, dt)
+    return O
+
+
+def moe_topk(logits, topk, bias=None, scoring="softmax", n_group=1, topk_group=1, group_top=1, renormalize=True,
+             scale=1.0, dtype=None, ids=None, out=None, stream=None):
+    """The experts of each token from router logits [T, E] (fp32/fp16/bf16): (ids int32 [T, topk], RW [T, topk]).
+
+    Scores are softmax or sigmoid of the logits; the experts are chosen by score + bias ([E] fp32) among the
+    topk_group best of n_group groups (a group's score: the sum of its group_top largest), in descending order, ties
+    to the lowest index; RW are the chosen scores, divided by their sum if renormalize, times scale, in `dtype`
+    (default: the logits' dtype).  Experts whose logit or bias is NaN or -inf come last, with weight 0."""
+    torch = _torch()
+    codes = {torch.float16: FP16, torch.bfloat16: BF16, torch.float32: FP32}
+    if scoring not in ("softmax", "sigmoid"):
+        raise ValueError("scoring must be 'softmax' or 'sigmoid', got %r" % (scoring,))
+    if logits.dim() != 2 or logits.dtype not in codes:
+        raise TypeError("logits must be [T, E] in fp32, fp16 or bf16")
+    _expect("logits", logits, logits.shape, logits.dtype, logits)
+    T, E = logits.shape
+    if dtype is None:
+        dtype = logits.dtype if out is None else out.dtype
+    if dtype not in codes:
+        raise TypeError("weights must be fp32, fp16 or bf16, got %s" % dtype)
+    if bias is not None:
+        _expect("bias", bias, (E,), torch.float32, logits)
+    if ids is None:
+        ids = torch.empty(T, int(topk), dtype=torch.int32, device=logits.device)
+    else:
+        _expect("ids", ids, (T, int(topk)), torch.int32, logits)
+    RW = _result(out, (T, int(topk)), dtype, logits)
+    _launch("ternocl_moe_topk", logits, stream, _ptr(logits), _ptr(bias), _ptr(ids), _ptr(RW), T, E, int(topk),
+            SCORE_SOFTMAX if scoring == "softmax" else SCORE_SIGMOID, int(n_group), int(topk_group), int(group_top),
+            int(bool(renormalize)), float(scale), codes[logits.dtype], codes[dtype])
+    return ids, RW

@@ -16,7 +16,7 @@ TERNOCL_OK = 0
 STATUS_NAMES = {0: "OK", 1: "ERR_SHAPE", 2: "ERR_ARG", 3: "ERR_CUDA", 4: "ERR_TIMEOUT",
                 5: "ERR_COMM", 6: "ERR_UNSUPPORTED", 7: "ERR_WORKSPACE"}
 
-vp, i32, sz, u64, f64 = C.c_void_p, C.c_int, C.c_size_t, C.c_uint64, C.c_double
+vp, i32, sz, u64, f64, f32 = C.c_void_p, C.c_int, C.c_size_t, C.c_uint64, C.c_double, C.c_float
 
 # name -> (restype, argtypes); must match include/ternocl.h
 SIGNATURES = {
@@ -54,6 +54,12 @@ SIGNATURES = {
     "ternocl_moe_decode_down": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp]),
     "ternocl_moe_decode_reduce": (i32, [vp, vp, i32, i32, i32, i32, vp]),
     "ternocl_moe_decode_down_sum": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp]),
+    "ternocl_int4_upcvt": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp]),
+    "ternocl_moe_gemm_int4": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp]),
+    "ternocl_moe_decode_gate_up_int4": (i32, [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp]),
+    "ternocl_moe_decode_down_sum_int4": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp]),
+    "ternocl_moe_topk": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, f32, i32, i32, vp]),
+    "ternocl_int4_pack": (i32, [vp, i32, i32, vp]),
     "ternocl_bitcos_random": (sz, [i32, i32, f64, u64, vp, sz]),
     "ternocl_bitcos_pack": (sz, [vp, i32, i32, vp, sz]),
     "ternocl_bitcos_slice_ranks": (i32, [vp, i32, i32, i32, vp]),

@@ -59,6 +59,7 @@ static size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 // shared memory a GEMV CTA may use (activation staging + weight ring)
 constexpr size_t kGemvSmemBudget = 100 * 1024;
 constexpr int kMaxClusterSK = 8;  // portable thread-block cluster size
+constexpr int kMaxGridYZ = 65535 * 8;  // rows whose 8-row blocks a grid's z extent holds
 
 // Split-K plan of a decode GEMV whose CTAs cover `cols` columns x `rows` activation
 // rows: enough CTAs to give every SM `per_sm` of them, each CTA keeping >= 1 group
@@ -198,6 +199,18 @@ static GemvPlan gemv_i8_plan(int M, int N, int K, bool allow_ws) {
     GemvPlan p = gemv_plan_t(M, N, K, 32, 8, 3, kMaxClusterSK, allow_ws, kGemvSmemBudget,
                              [&](int sk) { return int8_gemv_smem(M, K, sk); });
     if (M > kGemvDigitMaxM) gemv_min_split(p, K);
+    return p;
+}
+
+// int4 GEMV (gemv_int4.cu): 32 columns x 8 rows per CTA; split-K within a cluster
+static GemvPlan gemv_i4_plan(int M, int N, int K) {
+    const int G = K / kGS, sms = sm_count();
+    const long long tiles = (long long)((N + 31) / 32) * ((M + 7) / 8);
+    GemvPlan p;
+    p.warps = tiles >= 4LL * sms ? 4 : 8;
+    p.SK = tiles < sms && G >= 2 ? 2 : 1;
+    while (p.SK < G && p.SK < kMaxClusterSK && int4_gemv_smem(M, K, p.SK, p.warps) > kGemvSmemBudget) ++p.SK;
+    p.cluster = p.SK > 1;
     return p;
 }
 
@@ -390,6 +403,10 @@ int ternocl_device_error(int reset) {
     if (read_device_error_moe_decode(&t, reset) != cudaSuccess) return -1;
     v |= t;
     if (read_device_error_gemv_bitcos_p(&t, reset) != cudaSuccess) return -1;
+    v |= t;
+    if (read_device_error_gemm_int4(&t, reset) != cudaSuccess) return -1;
+    v |= t;
+    if (read_device_error_moe_decode_int4(&t, reset) != cudaSuccess) return -1;
     v |= t;
     return (int)v;
 }
@@ -740,6 +757,109 @@ int ternocl_moe_decode_down_sum(const int32_t *ids, const void *H, const void *R
     if (moe_decode_smem(K / kGS, topk, 2) > 227 * 1024) return TERNOCL_ERR_SHAPE;
     return cuda_status(moe_decode_down_sum_launch(ids, H, RW, B, S, O, T, N, K, topk, num_experts, dtype,
                                                   (cudaStream_t)stream));
+}
+
+// ---- 4-bit weights ----
+int ternocl_int4_upcvt(const void *A, const uint32_t *B, const void *S, void *C, const void *Other, const void *Bias,
+                       int M, int N, int K, int dtype, int postop, int out_f32, int algo, void *stream) {
+    int st = check_gemm_common(A, B, S, C, Other, Bias, M, N, K, dtype, postop, out_f32);
+    if (st != TERNOCL_OK) return st;
+    if (algo < TERNOCL_ALGO_AUTO || algo > TERNOCL_ALGO_GEMM) return TERNOCL_ERR_ARG;
+    if (M > kMaxGridYZ) return TERNOCL_ERR_SHAPE;
+    if (M == 0) return TERNOCL_OK;
+    GemvArgs a;
+    a.A = A; a.B = B; a.S = S; a.C = C; a.Other = Other; a.Bias = Bias;
+    a.M = M; a.N = N; a.K = K; a.dtype = dtype; a.postop = postop; a.out_f32 = out_f32;
+    a.stream = (cudaStream_t)stream;
+    if (algo == TERNOCL_ALGO_GEMM || (algo == TERNOCL_ALGO_AUTO && M > kInt4GemvMaxM))
+        return cuda_status(int4_gemm_launch(a, sm_count()));
+    const GemvPlan p = gemv_i4_plan(M, N, K);
+    if (int4_gemv_smem(M, K, p.SK, p.warps) > 227 * 1024) {
+        // (a K of more than 70,000 at M = 8: the GEMM walks any K)
+        if (algo == TERNOCL_ALGO_GEMV) return TERNOCL_ERR_WORKSPACE;
+        return cuda_status(int4_gemm_launch(a, sm_count()));
+    }
+    a.SK = p.SK;
+    a.warps = p.warps;
+    a.cluster = p.cluster ? 1 : 0;
+    return cuda_status(int4_gemv_launch(a));
+}
+
+int ternocl_moe_gemm_int4(const int32_t *meta, const void *A_all, const uint32_t *B_all, const void *S_all,
+                          void *C_all, const void *Other_all, int G, int N, int K, int num_experts, int dtype,
+                          int postop, int out_f32, void *stream) {
+    int st = check_gemm_common(A_all, B_all, S_all, C_all, Other_all, nullptr, G, N, K, dtype,
+                               postop == TERNOCL_POSTOP_BIAS ? TERNOCL_POSTOP_NONE : postop, out_f32);
+    if (st != TERNOCL_OK) return st;
+    if (postop == TERNOCL_POSTOP_BIAS) return TERNOCL_ERR_ARG;
+    if (!meta || num_experts < 1 || num_experts > 1024) return TERNOCL_ERR_ARG;
+    // the weights' rows are one tensor map's (32-bit coordinates), the row tiles a grid's
+    if ((long long)num_experts * (K / 8) > 0x7fffffffLL || G > (1 << 20)) return TERNOCL_ERR_SHAPE;
+    if (G == 0) return TERNOCL_OK;
+    GemvArgs a;
+    a.A = A_all; a.B = B_all; a.S = S_all; a.C = C_all; a.Other = Other_all;
+    a.M = G; a.N = N; a.K = K; a.dtype = dtype; a.postop = postop; a.out_f32 = out_f32;
+    a.stream = (cudaStream_t)stream;
+    return cuda_status(int4_gemm_launch(a, sm_count(), meta, num_experts));
+}
+
+int ternocl_moe_decode_gate_up_int4(const int32_t *ids, const void *X, const uint32_t *Bg, const void *Sg,
+                                    const uint32_t *Bu, const void *Su, void *H, int G, int N, int K, int topk,
+                                    int num_experts, int dtype, void *stream) {
+    int st = check_moe_decode(dtype, G, N, K, topk, num_experts);
+    if (st != TERNOCL_OK) return st;
+    if (G % topk || (long long)G * ((N + 31) / 32) > 0x7fffffffLL) return TERNOCL_ERR_SHAPE;
+    if (G == 0) return TERNOCL_OK;
+    if (!ids || !X || !Bg || !Sg || !Bu || !Su || !H) return TERNOCL_ERR_ARG;
+    if (!aligned(X, 16) || !aligned(Bg, 16) || !aligned(Bu, 16) || !aligned(Sg, 16) || !aligned(Su, 16) ||
+        !aligned(H, 2) || !aligned(ids, 4))
+        return TERNOCL_ERR_ARG;
+    return cuda_status(moe_decode_gate_up_int4_launch(ids, X, Bg, Sg, Bu, Su, H, G, N, K, topk, num_experts, dtype,
+                                                      (cudaStream_t)stream));
+}
+
+int ternocl_moe_decode_down_sum_int4(const int32_t *ids, const void *H, const void *RW, const uint32_t *B,
+                                     const void *S, void *O, int T, int N, int K, int topk, int num_experts,
+                                     int dtype, void *stream) {
+    int st = check_moe_decode(dtype, T, N, K, topk, num_experts);
+    if (st != TERNOCL_OK) return st;
+    if ((long long)T * ((N + 31) / 32) > 0x7fffffffLL || (long long)topk * (K / kGS) > 0x7fffffffLL ||
+        (long long)T * topk > 0x7fffffffLL)
+        return TERNOCL_ERR_SHAPE;
+    if (T == 0) return TERNOCL_OK;
+    if (!ids || !H || !RW || !B || !S || !O) return TERNOCL_ERR_ARG;
+    if (!aligned(H, 16) || !aligned(B, 16) || !aligned(S, 16) || !aligned(RW, 2) || !aligned(O, 2) ||
+        !aligned(ids, 4))
+        return TERNOCL_ERR_ARG;
+    return cuda_status(moe_decode_down_sum_int4_launch(ids, H, RW, B, S, O, T, N, K, topk, num_experts, dtype,
+                                                       (cudaStream_t)stream));
+}
+
+// ---- the experts' choice ----
+int ternocl_moe_topk(const void *logits, const float *bias, int32_t *ids, void *RW, int T, int E, int topk,
+                     int scoring, int n_group, int topk_group, int group_top, int renormalize, float scale,
+                     int logits_dtype, int rw_dtype, void *stream) {
+    auto dt_ok = [](int d) { return d == TERNOCL_FP16 || d == TERNOCL_BF16 || d == TERNOCL_FP32; };
+    auto size = [](int d) { return d == TERNOCL_FP32 ? 4u : 2u; };
+    if (!dt_ok(logits_dtype) || !dt_ok(rw_dtype)) return TERNOCL_ERR_ARG;
+    if (scoring != TERNOCL_SCORE_SOFTMAX && scoring != TERNOCL_SCORE_SIGMOID) return TERNOCL_ERR_ARG;
+    if (renormalize != 0 && renormalize != 1) return TERNOCL_ERR_ARG;
+    if (T < 0 || E < 1 || E > 1024 || topk < 1 || topk > 32) return TERNOCL_ERR_SHAPE;
+    if (n_group < 1 || n_group > 32 || E % n_group || topk_group < 1 || topk_group > n_group) return TERNOCL_ERR_SHAPE;
+    if (group_top < 1 || group_top > 2 || group_top > E / n_group) return TERNOCL_ERR_SHAPE;
+    if (topk > topk_group * (E / n_group)) return TERNOCL_ERR_SHAPE;
+    if (T == 0) return TERNOCL_OK;
+    if (!logits || !ids || !RW) return TERNOCL_ERR_ARG;
+    if (!aligned(logits, size(logits_dtype)) || !aligned(RW, size(rw_dtype)) || !aligned(ids, 4) ||
+        (bias && !aligned(bias, 4)))
+        return TERNOCL_ERR_ARG;
+    MoeTopkArgs a;
+    a.logits = logits; a.bias = bias; a.ids = ids; a.RW = RW;
+    a.T = T; a.E = E; a.topk = topk; a.scoring = scoring;
+    a.n_group = n_group; a.topk_group = topk_group; a.group_top = group_top;
+    a.renorm = renormalize; a.scale = scale; a.logits_dtype = logits_dtype; a.rw_dtype = rw_dtype;
+    a.stream = (cudaStream_t)stream;
+    return cuda_status(moe_topk_launch(a));
 }
 
 }  // extern "C"

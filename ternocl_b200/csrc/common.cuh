@@ -47,11 +47,15 @@ __device__ __forceinline__ float sigmoid_x(float x) {
     return x <= -10.0f ? 0.0f : __fdividef(1.0f, __expf(-x) + 1.0f);
 }
 
-template <int POSTOP>
+// the same within one fp32 ulp or two at every x, for fp32 outputs that show the difference
+// (__expf's error grows with |x|: 2^-22 relative at x = -8)
+__device__ __forceinline__ float sigmoid_accurate(float x) { return x <= -10.0f ? 0.0f : 1.0f / (expf(-x) + 1.0f); }
+
+template <int POSTOP, bool ACCURATE = false>
 __device__ __forceinline__ float epi(float v, float e) {
-    if constexpr (POSTOP == 1) return v * sigmoid_x(v) * e;
+    if constexpr (POSTOP == 1) return v * (ACCURATE ? sigmoid_accurate(v) : sigmoid_x(v)) * e;
     else if constexpr (POSTOP == 2 || POSTOP == 3) return v + e;
-    else if constexpr (POSTOP == 4) return sigmoid_x(v);
+    else if constexpr (POSTOP == 4) return ACCURATE ? sigmoid_accurate(v) : sigmoid_x(v);
     else return v;
 }
 
@@ -79,21 +83,21 @@ __device__ __forceinline__ void epi_store(void *__restrict__ C, const uint16_t *
 }
 
 // Two adjacent columns (n, n+1) of row m: one 32-bit (DT) or 64-bit (fp32) store.
-template <class DT, int POSTOP, bool OUT_F32>
+template <class DT, int POSTOP, bool OUT_F32, bool ACCURATE = false>
 __device__ __forceinline__ void epi_store2(void *__restrict__ C, const uint16_t *__restrict__ other,
                                            const void *__restrict__ bias, int N, int m, int n,
                                            float v0, float v1) {
     const size_t i = (size_t)m * N + n;
     if constexpr (POSTOP == 1 || POSTOP == 2) {
         const uint32_t o = *reinterpret_cast<const uint32_t *>(other + i);
-        v0 = epi<POSTOP>(v0, DT::tof((uint16_t)(o & 0xffffu)));
-        v1 = epi<POSTOP>(v1, DT::tof((uint16_t)(o >> 16)));
+        v0 = epi<POSTOP, ACCURATE>(v0, DT::tof((uint16_t)(o & 0xffffu)));
+        v1 = epi<POSTOP, ACCURATE>(v1, DT::tof((uint16_t)(o >> 16)));
     } else if constexpr (POSTOP == 3) {
-        v0 = epi<POSTOP>(v0, epi_in<DT, POSTOP, OUT_F32>(other, bias, i, n));
-        v1 = epi<POSTOP>(v1, epi_in<DT, POSTOP, OUT_F32>(other, bias, i + 1, n + 1));
+        v0 = epi<POSTOP, ACCURATE>(v0, epi_in<DT, POSTOP, OUT_F32>(other, bias, i, n));
+        v1 = epi<POSTOP, ACCURATE>(v1, epi_in<DT, POSTOP, OUT_F32>(other, bias, i + 1, n + 1));
     } else {
-        v0 = epi<POSTOP>(v0, 0.0f);
-        v1 = epi<POSTOP>(v1, 0.0f);
+        v0 = epi<POSTOP, ACCURATE>(v0, 0.0f);
+        v1 = epi<POSTOP, ACCURATE>(v1, 0.0f);
     }
     if constexpr (OUT_F32) {
         *reinterpret_cast<float2 *>(reinterpret_cast<float *>(C) + i) = make_float2(v0, v1);

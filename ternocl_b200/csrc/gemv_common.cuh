@@ -197,6 +197,17 @@ inline size_t smem_bytes_w(int warps, int rows, int krange) {
                        : warps >= 8 ? smem_bytes<Policy, 8>(rows, krange) : smem_bytes<Policy, 4>(rows, krange);
 }
 
+// A policy that declares the type AccurateEpilogueTag has the sigmoid of its fp32 outputs computed to
+// fp32 accuracy (sigmoid_accurate).
+template <class ColMap, class = void>
+struct AccurateEpilogue {
+    static constexpr bool value = false;
+};
+template <class ColMap>
+struct AccurateEpilogue<ColMap, std::void_t<typename ColMap::AccurateEpilogueTag>> {
+    static constexpr bool value = true;
+};
+
 // Reduction over the CTA's K-split warps (in warp order, through `smem`, >= 8 KB),
 // then over the SK CTAs of the strip (cluster DSMEM or workspace, in split order),
 // and the epilogue store.  v[h*4 + i] = this thread's partial for activation row
@@ -210,6 +221,7 @@ __device__ __forceinline__ void finish(const Params &p, char *smem, float v[8], 
     const int n0 = blockIdx.x * 32;
     const int mb = blockIdx.z * 8;
     const int sk = blockIdx.y;
+    constexpr bool kAcc = OUT_F32 && AccurateEpilogue<ColMap>::value;
     float(*red)[32][8] = reinterpret_cast<float(*)[32][8]>(smem);  // [W][lane][8]
     if (warp > 0) {
 #pragma unroll
@@ -247,8 +259,8 @@ __device__ __forceinline__ void finish(const Params &p, char *smem, float v[8], 
             const int m = mb + 2 * q + h;
             if (m < p.M) {
                 if (ColMap::kContiguousCols) {
-                    epi_store2<DT, POSTOP, OUT_F32>(p.C, p.Other, p.Bias, p.N, m, cols[0], v[4 * h], v[4 * h + 1]);
-                    epi_store2<DT, POSTOP, OUT_F32>(p.C, p.Other, p.Bias, p.N, m, cols[2], v[4 * h + 2], v[4 * h + 3]);
+                    epi_store2<DT, POSTOP, OUT_F32, kAcc>(p.C, p.Other, p.Bias, p.N, m, cols[0], v[4 * h], v[4 * h + 1]);
+                    epi_store2<DT, POSTOP, OUT_F32, kAcc>(p.C, p.Other, p.Bias, p.N, m, cols[2], v[4 * h + 2], v[4 * h + 3]);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)

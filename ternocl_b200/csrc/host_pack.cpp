@@ -129,6 +129,24 @@ int ternocl_bitcos_slice_ranks(const uint32_t *buf, int K, int N, int ls, uint32
     return TERNOCL_OK;
 }
 
+int ternocl_int4_pack(const int8_t *codes, int K, int N, uint32_t *out) {
+    if (!codes || !out) return TERNOCL_ERR_ARG;
+    if (K <= 0 || N <= 0 || K % 8) return TERNOCL_ERR_SHAPE;
+    int bad = 0;
+#pragma omp parallel for reduction(| : bad)
+    for (int kp = 0; kp < K / 8; ++kp)
+        for (int n = 0; n < N; ++n) {
+            uint32_t w = 0;
+            for (int j = 0; j < 8; ++j) {
+                const int c = codes[((size_t)kp * 8 + j) * N + n];
+                bad |= c < -8 || c > 7;
+                w |= ((uint32_t)c & 15u) << (4 * j);
+            }
+            out[(size_t)kp * N + n] = w;
+        }
+    return bad ? TERNOCL_ERR_ARG : TERNOCL_OK;
+}
+
 int ternocl_int1_to_sel(const uint32_t *B, uint32_t *out, int K, int N) {
     if (!B || !out) return TERNOCL_ERR_ARG;
     if (K <= 0 || N <= 0 || K % 32 || N % 16) return TERNOCL_ERR_SHAPE;

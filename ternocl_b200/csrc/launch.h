@@ -206,6 +206,33 @@ cudaError_t moe_decode_down_sum_launch(const int *ids, const void *H, const void
                                        cudaStream_t st);
 cudaError_t moe_decode_reduce_launch(const float *Y, void *O, int T, int N, int topk, int dtype, cudaStream_t st);
 cudaError_t read_device_error_moe_decode(unsigned *out, int reset);
+// the experts' choice from router logits (moe_topk.cu)
+struct MoeTopkArgs {
+    const void *logits = nullptr;
+    const float *bias = nullptr;
+    int *ids = nullptr;
+    void *RW = nullptr;
+    int T = 0, E = 0, topk = 0, scoring = 0, n_group = 1, topk_group = 1, group_top = 1, renorm = 0;
+    float scale = 1.0f;
+    int logits_dtype = 0, rw_dtype = 0;
+    cudaStream_t stream = nullptr;
+};
+cudaError_t moe_topk_launch(const MoeTopkArgs &a);
+// int4 GEMV (gemv_int4.cu), GEMM (gemm_int4.cu; grouped with meta) and MoE decode GEMVs
+// (moe_decode_int4.cu)
+size_t int4_gemv_smem(int M, int K, int SK, int warps);
+cudaError_t int4_gemv_launch(const GemvArgs &a);
+cudaError_t int4_gemm_launch(const GemvArgs &a, int sms, const int *meta = nullptr, int E = 0);
+cudaError_t read_device_error_gemm_int4(unsigned *out, int reset);
+cudaError_t moe_decode_gate_up_int4_launch(const int *ids, const void *X, const uint32_t *Bg, const void *Sg,
+                                           const uint32_t *Bu, const void *Su, void *H, int G, int N, int K, int topk,
+                                           int E, int dtype, cudaStream_t st);
+cudaError_t moe_decode_down_sum_int4_launch(const int *ids, const void *H, const void *RW, const uint32_t *B,
+                                            const void *S, void *O, int T, int N, int K, int topk, int E, int dtype,
+                                            cudaStream_t st);
+cudaError_t read_device_error_moe_decode_int4(unsigned *out, int reset);
+// largest M that TERNOCL_ALGO_AUTO gives the int4 GEMV
+constexpr int kInt4GemvMaxM = 8;
 // M from which TERNOCL_ALGO_AUTO picks the GEMM (int2_fp16_upcvt/main.cpp:160)
 constexpr int kGemmMinM = 64;
 // split-K factor the register-decode GEMV's planner picks when a workspace exists

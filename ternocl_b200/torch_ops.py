@@ -11,11 +11,14 @@ operator without running it.  The activation may carry leading batch dimensions
   int2_linear / int1_linear   ternocl_int2_upcvt / ternocl_int1_upcvt
   bitcos_linear               ternocl_bitcos_upcvt
   bitcos_hadamard_linear      ternocl_bitcos_upcvt_hadamard
+  int4_linear                 ternocl_int4_upcvt
   int8_linear                 ternocl_int8_quant_a + ternocl_int2_int8 (qmode 0)
   hadamard                    ternocl_hadamard_fwht
   moe_prefill                 route, gather (or quant + gather_q), up, gate (SiLU x up),
                               down, combine: the int2_moe/prefill.cpp layer
   moe_decode                  gate_up + down_sum: the int2_moe/main.cpp layer (--fused)
+  moe_topk                    ternocl_moe_topk: the ids and weights of the layers' arguments
+  moe_prefill_int4, moe_decode_int4   the same layers with 4-bit experts
 """
 from typing import Optional
 
@@ -162,5 +165,74 @@ def moe_decode(X: torch.Tensor, ids: torch.Tensor, RW: torch.Tensor, Bg: torch.T
 
 
 @moe_decode.register_fake
+def _(X, ids, RW, Bg, Sg, Bu, Su, Bd, Sd, num_experts, topk):
+    return torch.empty_like(X)
+
+
+# ---- 4-bit weights and the experts' choice ---------------------------------------------
+@torch.library.custom_op(_NS + "::int4_linear", mutates_args=())
+def int4_linear(A: torch.Tensor, B: torch.Tensor, S: torch.Tensor, postop: int = 0, out_f32: bool = False,
+                other: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """C = epi(A @ dequant_int4(B, S)); B int32 [K/8, N], S [K/128, N]."""
+    C = tl.int4_upcvt(_rows(A), B, S, postop=postop, out_f32=out_f32,
+                      other=None if other is None else _rows(other), bias=bias)
+    return C.reshape(*A.shape[:-1], B.shape[1])
+
+
+@int4_linear.register_fake
+def _(A, B, S, postop=0, out_f32=False, other=None, bias=None):
+    return _fake_linear(A, B.shape[1], out_f32)
+
+
+@torch.library.custom_op(_NS + "::moe_topk", mutates_args=())
+def moe_topk(logits: torch.Tensor, topk: int, bias: Optional[torch.Tensor] = None, scoring: str = "softmax",
+             n_group: int = 1, topk_group: int = 1, group_top: int = 1, renormalize: bool = True, scale: float = 1.0,
+             dtype: Optional[torch.dtype] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(ids int32 [..., topk], weights [..., topk]) of router logits [..., E]; see ternocl_b200.moe_topk."""
+    ids, RW = tl.moe_topk(_rows(logits), topk, bias=bias, scoring=scoring, n_group=n_group, topk_group=topk_group,
+                          group_top=group_top, renormalize=renormalize, scale=scale, dtype=dtype)
+    shape = (*logits.shape[:-1], topk)
+    return ids.reshape(shape), RW.reshape(shape)
+
+
+@moe_topk.register_fake
+def _(logits, topk, bias=None, scoring="softmax", n_group=1, topk_group=1, group_top=1, renormalize=True, scale=1.0,
+      dtype=None):
+    shape = (*logits.shape[:-1], topk)
+    return logits.new_empty(shape, dtype=torch.int32), logits.new_empty(shape, dtype=dtype or logits.dtype)
+
+
+@torch.library.custom_op(_NS + "::moe_prefill_int4", mutates_args=())
+def moe_prefill_int4(X: torch.Tensor, ids: torch.Tensor, RW: torch.Tensor, Bg: torch.Tensor, Sg: torch.Tensor,
+                     Bu: torch.Tensor, Su: torch.Tensor, Bd: torch.Tensor, Sd: torch.Tensor, num_experts: int,
+                     topk: int) -> torch.Tensor:
+    """moe_prefill with 4-bit experts: B* int32 [E, K/8, N], S* [E, K/128, N]."""
+    X2 = _rows(X)
+    meta, perm, inv = tl.moe_route(ids.reshape(-1).contiguous(), num_experts)
+    Xs = tl.moe_gather(X2, perm, topk)
+    up = tl.moe_gemm_int4(meta, Xs, Bu, Su, num_experts)
+    H = tl.moe_gemm_int4(meta, Xs, Bg, Sg, num_experts, postop=1, other=up)
+    Y = tl.moe_gemm_int4(meta, H, Bd, Sd, num_experts, out_f32=True)
+    return tl.moe_combine(Y, inv, RW.reshape(-1).contiguous(), X2.shape[0], topk).reshape(X.shape)
+
+
+@moe_prefill_int4.register_fake
+def _(X, ids, RW, Bg, Sg, Bu, Su, Bd, Sd, num_experts, topk):
+    return torch.empty_like(X)
+
+
+@torch.library.custom_op(_NS + "::moe_decode_int4", mutates_args=())
+def moe_decode_int4(X: torch.Tensor, ids: torch.Tensor, RW: torch.Tensor, Bg: torch.Tensor, Sg: torch.Tensor,
+                    Bu: torch.Tensor, Su: torch.Tensor, Bd: torch.Tensor, Sd: torch.Tensor, num_experts: int,
+                    topk: int) -> torch.Tensor:
+    """moe_decode with 4-bit experts."""
+    X2 = _rows(X)
+    ids1 = ids.reshape(-1).contiguous()
+    H = tl.moe_decode_gate_up_int4(ids1, X2, Bg, Sg, Bu, Su, num_experts, topk)
+    return tl.moe_decode_down_sum_int4(ids1, H, RW.reshape(-1).contiguous(), Bd, Sd, num_experts,
+                                       topk).reshape(X.shape)
+
+
+@moe_decode_int4.register_fake
 def _(X, ids, RW, Bg, Sg, Bu, Su, Bd, Sd, num_experts, topk):
     return torch.empty_like(X)

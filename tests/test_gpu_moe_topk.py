@@ -1,0 +1,138 @@
+"""The experts' choice on the GPU against its 64-bit definition (int4_ref.topk64): ids equal, weights within
+the rounding of their type (the kernel computes them in 64 bits or with a few fp32 operations: 2^-20)."""
+import itertools
+
+import numpy as np
+import pytest
+import torch
+
+from int4_ref import topk64
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def run(tl, logits, topk, dtype=torch.float32, **how):
+    ids, w = tl.moe_topk(logits, topk, dtype=dtype, **how)
+    T, E = logits.shape
+    assert ids.shape == w.shape == (T, topk) and ids.dtype == torch.int32 and w.dtype == dtype
+    if how.get("bias") is not None:
+        how = {**how, "bias": how["bias"].cpu().numpy()}
+    want_ids, want_w = topk64(logits.double().cpu().numpy(), topk, **how)
+    got = ids.cpu().numpy()
+    assert np.array_equal(got, want_ids), np.argwhere((got != want_ids).any(1))[:4]
+    err = np.abs(w.double().cpu().numpy() - want_w)
+    info = torch.finfo(dtype)
+    assert np.all(err <= np.abs(want_w) * (info.eps / 2 + 2.0 ** -20) + info.tiny * info.eps), err.max()
+
+
+@pytest.mark.parametrize("T,E,topk", [(1, 1, 1), (1, 8, 8), (5, 31, 4), (3, 33, 32), (130, 64, 6), (77, 100, 1),
+                                      (9, 128, 8), (64, 256, 8), (7, 500, 17), (6, 1024, 32)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("biased", [False, True])
+def test_shapes(cuda, tl, T, E, topk, scoring, biased):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(T + E)
+    for k, dtype in enumerate(TYPES):
+        logits = (2.0 * torch.randn(T, E, generator=g, device="cuda")).to(dtype)
+        bias = 0.1 * torch.randn(E, generator=g, device="cuda") if biased else None
+        run(tl, logits, topk, dtype=TYPES[(k + E) % 3], bias=bias, scoring=scoring, renormalize=bool(k & 1),
+            scale=[1.0, 2.5][k & 1])
+
+
+@pytest.mark.parametrize("E,n_group,topk_group,topk", [(8, 2, 1, 4), (256, 8, 4, 8), (160, 8, 3, 6), (96, 32, 5, 12),
+                                                        (64, 4, 4, 9), (60, 3, 2, 32)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("group_top", [1, 2])
+def test_groups(cuda, tl, E, n_group, topk_group, topk, scoring, group_top):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(E)
+    for biased in (False, True):
+        logits = 2.0 * torch.randn(41, E, generator=g, device="cuda")
+        bias = 0.1 * torch.randn(E, generator=g, device="cuda") if biased else None
+        run(tl, logits, topk, bias=bias, scoring=scoring, n_group=n_group, topk_group=topk_group, group_top=group_top)
+
+
+def test_ties_go_to_the_lowest_index(cuda, tl):
+    for E, dtype in itertools.product((7, 64, 300), TYPES):
+        g = torch.Generator(device="cuda")
+        g.manual_seed(E)
+        logits = torch.randint(-2, 3, (50, E), generator=g, device="cuda").to(dtype)
+        logits[0] = 0.0
+        logits[1, ::2] = -0.0
+        logits[1, 1::2] = 0.0
+        for scoring in ("softmax", "sigmoid"):
+            run(tl, logits, min(E, 9), scoring=scoring)
+            run(tl, logits, min(E, 9), scoring=scoring, bias=torch.zeros(E, device="cuda"))
+    run(tl, torch.zeros(3, 32, device="cuda"), 5, n_group=8, topk_group=2, group_top=2, scoring="sigmoid")
+
+
+def test_masked_and_extreme_logits(cuda, tl):
+    inf, nan = float("inf"), float("nan")
+    E = 24
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    base = torch.randn(12, E, generator=g, device="cuda")
+    base[0] = -inf                       # a row with nothing
+    base[1] = nan
+    base[2, 3:] = -inf                   # fewer unmasked than topk
+    base[3, 5] = nan
+    base[4, 7] = inf
+    base[5, 2] = base[5, 9] = inf
+    base[6] = torch.finfo(torch.float32).min
+    base[7] = torch.linspace(-3e38, 3e38, E)
+    base[8] = 1e4 * base[8]
+    base[9, ::2] = -inf
+    bias = torch.zeros(E, device="cuda")
+    bias[4], bias[6], bias[8] = -inf, nan, 0.3
+    for scoring, renorm in itertools.product(("softmax", "sigmoid"), (False, True)):
+        run(tl, base, 8, scoring=scoring, renormalize=renorm)
+        run(tl, base[:8], 8, scoring=scoring, renormalize=renorm, n_group=4, topk_group=2, group_top=2)
+        run(tl, base[:6], 8, scoring=scoring, renormalize=renorm, bias=bias)
+        run(tl, base[:6], 8, scoring=scoring, renormalize=renorm, bias=bias, n_group=6, topk_group=3, group_top=1)
+    run(tl, base[:6].half(), 8, dtype=torch.float16)
+    for value in (inf, -inf):
+        b = torch.zeros(E, device="cuda")
+        b[11] = value
+        run(tl, torch.randn(5, E, generator=g, device="cuda"), 4, bias=b, scoring="sigmoid")
+
+
+def test_near_ties_are_told_apart(cuda, tl):
+    """Choice values that differ by a few 2^-40 of themselves (equal in 32 bits) keep their 64-bit order."""
+    E = 64
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    logits = torch.randn(200, E, generator=g, device="cuda")
+    for scoring in ("softmax", "sigmoid"):
+        x = logits.double()
+        s = torch.softmax(x, 1) if scoring == "softmax" else torch.sigmoid(x)
+        # the bias that makes the first row's choice values 1 up to the bias's own rounding to 32 bits
+        run(tl, logits, 8, bias=(1.0 - s[0]).float(), scoring=scoring)
+        # one fp32 step between neighbouring logits
+        step = torch.full((4, E), 1.25, device="cuda").view(torch.int32) + torch.randperm(E, device="cuda").int()
+        run(tl, step.view(torch.float32), 8, scoring=scoring)
+        run(tl, step.view(torch.float32), 8, bias=torch.full((E,), 0.5, device="cuda"), scoring=scoring)
+
+
+def test_long_batches_streams_and_graphs(cuda, tl):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(4)
+    logits = torch.randn(5003, 256, generator=g, device="cuda")
+    bias = 0.05 * torch.randn(256, generator=g, device="cuda")
+    how = dict(bias=bias, scoring="sigmoid", n_group=8, topk_group=4, group_top=2)
+    run(tl, logits, 8, **how)
+    ids, w = tl.moe_topk(logits, 8, dtype=torch.bfloat16, **how)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ids2, w2 = tl.moe_topk(logits, 8, dtype=torch.bfloat16, **how)
+    side.synchronize()
+    assert torch.equal(ids, ids2) and torch.equal(w, w2)
+    x, i3, w3 = torch.zeros_like(logits), torch.empty_like(ids), torch.empty_like(w)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tl.moe_topk(x, 8, ids=i3, out=w3, **how)
+    x.copy_(logits)
+    graph.replay()
+    assert torch.equal(ids, i3) and torch.equal(w, w3)
+    assert tl.moe_topk(logits[:0], 8, **how)[0].shape == (0, 8)
