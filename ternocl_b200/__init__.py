@@ -369,32 +369,44 @@ def moe_decode_down_sum(ids, H, RW, B, S, num_experts, topk, out=None, stream=No
 
 
 # ---- 4-bit weights and the experts' choice ------------------------------------------------
+# These functions check every shape and type; a decode step makes hundreds of such calls, so
+# the checks of a correct call are a few attribute reads, and only a wrong one looks closer.
+def _raw_stream(device):
+    """Handle of torch's current stream on CUDA device index `device`."""
+    torch = _torch()
+    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # 3 us less than the Stream object
+    return get(device) if get is not None else torch.cuda.current_stream(device).cuda_stream
+
+
 def _launch(name, like, stream, *args):
     """Call entry point `name` on `like`'s device (made current for the call if it is not); no rows, no call."""
     torch = _torch()
     if like.shape[0] == 0:
-        return None
-    if like.device.index == torch.cuda.current_device():
-        return call(name, *args, _stream(stream))
-    with torch.cuda.device(like.device):
-        return call(name, *args, _stream(stream))
+        return
+    device = like.get_device()
+    s = _raw_stream(device) if stream is None else _stream(stream)
+    if device == torch.cuda.current_device():
+        call(name, *args, s)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, s)
 
 
 def _expect(name, t, shape, dtype, like):
     """`t` is a contiguous CUDA tensor of this shape and dtype on `like`'s device."""
+    if t.is_cuda and t.get_device() == like.get_device() and t.shape == shape and t.dtype == dtype and t.is_contiguous():
+        return
     if not t.is_cuda or not t.is_contiguous() or t.device != like.device:
         raise ValueError("%s must be a contiguous CUDA tensor on %s" % (name, like.device))
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
-    if t.dtype != dtype:
-        raise TypeError("%s must be %s, got %s" % (name, dtype, t.dtype))
+    raise TypeError("%s must be %s, got %s" % (name, dtype, t.dtype))
 
 
 def _expect_int4(name, B, S, lead, K, N, like):
-    torch = _torch()
     if K % 128 or N % 16:
         raise ValueError("%s: K %% 128 == 0 and N %% 16 == 0 needed, got K = %d, N = %d" % (name, K, N))
-    _expect(name, B, (*lead, K // 8, N), torch.int32, like)
+    _expect(name, B, (*lead, K // 8, N), _torch().int32, like)
     _expect("the scales of " + name, S, (*lead, K // 128, N), like.dtype, like)
 
 
@@ -402,27 +414,29 @@ def _rows2(name, A):
     if A.dim() != 2:
         raise ValueError("%s must be [rows, K], got %s" % (name, tuple(A.shape)))
     _expect(name, A, A.shape, A.dtype, A)
-    return dtype_code(A), A.shape[0], A.shape[1]
+    M, K = A.shape
+    return dtype_code(A), M, K
 
 
 def _result(out, shape, dtype, like):
     if out is None:
-        return _torch().empty(shape, dtype=dtype, device=like.device)
+        return like.new_empty(shape, dtype=dtype)
     _expect("out", out, shape, dtype, like)
     return out
 
 
 def _int4_epilogue(A, M, N, postop, out_f32, other, bias):
-    torch = _torch()
+    """Checks the epilogue's operands; the output's dtype."""
+    dtype = _torch().float32 if out_f32 else A.dtype
     if postop in (POSTOP_SILU_MUL, POSTOP_ADD):
         if other is None:
             raise ValueError("postop %d needs other" % postop)
         _expect("other", other, (M, N), A.dtype, A)
-    if postop == POSTOP_BIAS:
+    elif postop == POSTOP_BIAS:
         if bias is None:
             raise ValueError("postop 3 needs bias")
-        _expect("bias", bias, (N,), torch.float32 if out_f32 else A.dtype, A)
-    return torch.float32 if out_f32 else A.dtype
+        _expect("bias", bias, (N,), dtype, A)
+    return dtype
 
 
 def int4_upcvt(A, B, S, postop=0, out_f32=False, other=None, bias=None, out=None, algo=0, stream=None):
@@ -497,6 +511,16 @@ def moe_decode_down_sum_int4(ids, H, RW, B, S, num_experts, topk, out=None, stre
     return O
 
 
+_TYPE_CODES = {}
+
+
+def _type_codes():
+    if not _TYPE_CODES:
+        torch = _torch()
+        _TYPE_CODES.update({torch.float16: FP16, torch.bfloat16: BF16, torch.float32: FP32})
+    return _TYPE_CODES
+
+
 def moe_topk(logits, topk, bias=None, scoring="softmax", n_group=1, topk_group=1, group_top=1, renormalize=True,
              scale=1.0, dtype=None, ids=None, out=None, stream=None):
     """The experts of each token from router logits [T, E] (fp32/fp16/bf16): (ids int32 [T, topk], RW [T, topk]).
@@ -506,7 +530,7 @@ def moe_topk(logits, topk, bias=None, scoring="softmax", n_group=1, topk_group=1
     to the lowest index; RW are the chosen scores, divided by their sum if renormalize, times scale, in `dtype`
     (default: the logits' dtype).  Experts whose logit or bias is NaN or -inf come last, with weight 0."""
     torch = _torch()
-    codes = {torch.float16: FP16, torch.bfloat16: BF16, torch.float32: FP32}
+    codes = _type_codes()
     if scoring not in ("softmax", "sigmoid"):
         raise ValueError("scoring must be 'softmax' or 'sigmoid', got %r" % (scoring,))
     if logits.dim() != 2 or logits.dtype not in codes:
@@ -520,7 +544,7 @@ def moe_topk(logits, topk, bias=None, scoring="softmax", n_group=1, topk_group=1
     if bias is not None:
         _expect("bias", bias, (E,), torch.float32, logits)
     if ids is None:
-        ids = torch.empty(T, int(topk), dtype=torch.int32, device=logits.device)
+        ids = logits.new_empty((T, int(topk)), dtype=torch.int32)
     else:
         _expect("ids", ids, (T, int(topk)), torch.int32, logits)
     RW = _result(out, (T, int(topk)), dtype, logits)

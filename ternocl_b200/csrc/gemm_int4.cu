@@ -10,23 +10,29 @@
 //
 // The weights are the MMA's M operand (128 columns n of C) and the activation rows its N
 // operand (up to MT): then a TMEM lane is a column n, a thread scales its whole lane by one
-// S[g,n], the N extent follows the rows that are there, and the accumulated tile's rows are
-// stored 32 consecutive columns per warp.
+// S[g,n], and the N extent follows the rows that are there.
 //
-// CTA: 128 columns x MT rows, groups [G sk/SK, G (sk+1)/SK) of a K split over a
-// thread-block cluster.  Roles:
-//   warp 0      TMA producer: per group two boxes of A (MT rows x 64, 128-byte swizzle) and
-//               one box of packed words (16 word rows x 128 columns);
-//   warp 1      TMEM allocation and the MMA issuer: per group 2 x 4 tcgen05.mma kind::f16
-//               (M=128, N=rows rounded up to 16, K=16) into one of kAccBufs accumulators;
-//   4 NT warps  decode (NT teams of 4): a team turns every NT-th half group (8 word rows) into
-//               a K=64 slice of the M operand, MN-major: one lane makes one 8 x 8 core
-//               matrix out of 8 words (8 columns of one word row);
-//   NP warps    promotion: tcgen05.ld of a finished group, acc += S * D_g, then the epilogue.
-// With SK > 1 the CTAs of a cluster leave their sums in shared memory and each adds up a
-// share of the rows in split order over distributed shared memory (deterministic).
-// Every mbarrier wait is bounded (tc::mbar_wait); on a timeout the roles skip ahead, the
-// producer waits (bounded) for its copies in flight, and TMEM is freed.
+// Persistent CTAs walk tiles of 128 columns x MT rows; a step is half a group (K = 64):
+//   warp 0      the activations of a step: TMA boxes of 64 rows x 64 (128-byte swizzle);
+//   warp 1      the MMA issuer: per step 4 tcgen05.mma kind::f16 (M=128, N=rows rounded up to
+//               16, K=16) into one of kAccBufs accumulators;
+//   warp 2      the packed words of a step: one TMA box of 8 word rows x 128 columns;
+//   warp 3      TMEM allocation;
+//   4 NT warps  decode, NT teams of 4 that take the steps in turn: one lane makes one 8 x 8 core
+//               matrix of the M operand (MN-major) out of 8 words;
+//   NP warps    promotion: tcgen05.ld of a finished group, acc += S * D_g (f32x2), and at the
+//               tile's end the epilogue, while the other roles run on into the next tile.
+// Few tiles split K over a thread-block cluster: its CTAs leave their sums in shared memory
+// and each adds up a share of the rows in split order over distributed shared memory.
+//
+// What bounds it: for many rows the MMAs (1024 cycles for a group at MT = 256) and, close
+// behind, the issue slots of decode and promotion; for few rows the decode, which all 16 (8)
+// decode warps of an SM share.  Chains of waits, not throughput, decided the design: a
+// step's decode takes ~1000 cycles from its words' arrival to the MMA, so NT teams keep NT
+// steps in flight, every stage has one barrier that says "filled" and one that says "free", and
+// the MMA issuer waits once per step.
+// Every mbarrier wait is bounded (tc::mbar_wait); on a timeout the roles stop, the producers
+// wait (bounded) for their copies in flight, and TMEM is freed.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -39,37 +45,63 @@
 namespace ternocl {
 namespace gemm4 {
 
-constexpr int BN = 128;                        // columns of C per CTA (the MMA's M)
-constexpr int kHalf = 64;                      // K rows of a decode stage
+constexpr int BN = 128;                        // columns of C per tile (the MMA's M)
+constexpr int kStepK = 64;                     // K rows of a step
 constexpr int kDecLBO = 128;                   // next 8 K rows
-constexpr int kDecSBO = kHalf / 8 * 128 + 16;  // next 8 columns; the pad spreads the stores over the banks
-constexpr int kDecStageBytes = BN / 8 * kDecSBO;
-constexpr int kPackBytes = int4::kWordsPerGroup * BN * 4;  // 8 KB
-constexpr int kMetaTile = 128;                 // rows of a tile in moe_route's meta
+constexpr int kDecSBO = kStepK / 8 * 128 + 16; // next 8 columns; the pad spreads the stores over the banks
+constexpr int kDecBytes = BN / 8 * kDecSBO;    // 16640
+constexpr int kWordBytes = kStepK / int4::kRowsPerWord * BN * 4;  // 4 KB
+constexpr int kMaxExperts = 1024;
 
+// Threads, rings and register shares by the rows of a tile.  kRegs*: setmaxnreg values (0: not
+// used), whose sum over the warps stays within what the block launches with.
 template <int MT_>
-struct Cfg {
-    static constexpr int MT = MT_;
-    static constexpr int NT = MT >= 128 ? 2 : 1;         // decode teams of 4 warps
-    static constexpr int NP = MT >= 128 ? 8 : 4;         // promotion warps
-    static constexpr int kWarps = 2 + 4 * NT + NP;
+struct Cfg;
+template <>
+struct Cfg<256> {
+    static constexpr int MT = 256, NT = 2, NP = 8, kSteps = 4, kWords = 6, kAccBufs = 2, kCtasPerSm = 1;
+    static constexpr int kRegsPromote = 168, kRegsOther = 48;
+};
+template <>
+struct Cfg<128> {
+    static constexpr int MT = 128, NT = 3, NP = 8, kSteps = 5, kWords = 6, kAccBufs = 4, kCtasPerSm = 1;
+    static constexpr int kRegsPromote = 112, kRegsOther = 64;
+};
+template <>
+struct Cfg<64> {
+    static constexpr int MT = 64, NT = 4, NP = 4, kSteps = 6, kWords = 8, kAccBufs = 4, kCtasPerSm = 1;
+    static constexpr int kRegsPromote = 112, kRegsOther = 72;
+};
+template <>
+struct Cfg<32> {
+    static constexpr int MT = 32, NT = 2, NP = 4, kSteps = 4, kWords = 4, kAccBufs = 4, kCtasPerSm = 2;
+    static constexpr int kRegsPromote = 0, kRegsOther = 0;
+};
+
+template <int MT>
+struct Plan : Cfg<MT> {
+    using C = Cfg<MT>;
+    static constexpr int kWarps = 4 + 4 * C::NT + C::NP;
     static constexpr int kThreads = kWarps * 32;
-    static constexpr int kCols = MT * 4 / NP;            // accumulator columns per promotion thread
-    static constexpr int kLoads = 3;
-    static constexpr int kDecs = MT >= 128 ? 5 : 3;
-    static constexpr int kAccBufs = MT >= 128 ? 4 : 2;
-    static constexpr int kTmemCols = MT * kAccBufs;
-    static constexpr int kABytes = MT * kGS * 2;
-    static constexpr int kCtasPerSm = MT >= 128 ? 1 : 2;
-    // shared memory: decoded stages first, then 1024-byte aligned A stages
-    static constexpr int dec = 0;
-    static constexpr int a = (kDecs * kDecStageBytes + 1023) / 1024 * 1024;
-    static constexpr int pack = a + kLoads * kABytes;
-    static constexpr int bars = pack + kLoads * kPackBytes;
-    static constexpr int total = bars + 256 + 1024;  // + alignment slack
+    static constexpr int kCols = MT * 4 / C::NP;  // accumulator columns per promotion thread
+    static constexpr int kTmemCols = MT * C::kAccBufs;
+    static constexpr int kBoxRows = MT < 64 ? MT : 64;
+    static constexpr int kBoxBytes = kBoxRows * kStepK * 2;
+    static constexpr int kABytes = MT * kStepK * 2;
+    static constexpr int kLaunchRegs = 65536 / kThreads / C::kCtasPerSm / 8 * 8;
+    static_assert(C::kRegsPromote * C::NP * 32 + C::kRegsOther * (kWarps - C::NP) * 32 <= kLaunchRegs * kThreads,
+                  "register shares");
+    // shared memory: 1024-byte aligned A stages first
+    static constexpr int a = 0;
+    static constexpr int dec = a + C::kSteps * kABytes;
+    static constexpr int words = dec + C::kSteps * kDecBytes;
+    static constexpr int bars = words + C::kWords * kWordBytes;
+    static constexpr int first = bars + 512;  // grouped: first tile of every expert
+    static constexpr int total = first + (kMaxExperts + 1) * 4 + 1024;  // + alignment slack
     static_assert(total <= 227 * 1024, "shared memory");
-    static_assert(MT * BN * 4 <= bars, "the split's sums reuse the stages");
-    static_assert(kTmemCols * kCtasPerSm <= 512, "TMEM");
+    static_assert(MT * BN * 4 <= words, "the split's sums reuse the stages");
+    static_assert(kTmemCols * C::kCtasPerSm <= 512 && (kTmemCols & (kTmemCols - 1)) == 0, "TMEM");
+    static_assert((2 * C::kSteps + 2 * C::kWords + 2 * C::kAccBufs) * 8 + 4 <= 512, "barriers");
 };
 
 struct Params {
@@ -77,31 +109,79 @@ struct Params {
     void *C;
     const uint16_t *Other;
     const void *Bias;
-    int M, N, K, SK;
-    const int *meta;  // grouped: [E+1 row offsets | E+1 row-tile offsets], else null
+    int M, N, K, SK, strips;
+    const int *meta;  // grouped: E+1 row offsets (moe_route's meta), else null
     int E;
 };
 
-// 8 words (columns 8nb..8nb+7 of one word row) -> the core matrix rows out[r] (K row r, the 8
-// columns as 4 half2): two columns' halves side by side decode together
-template <class DT>
-__device__ __forceinline__ void decode8(const uint4 w0, const uint4 w1, uint4 (&out)[8]) {
-    const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-    uint32_t d[4][8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t z = __byte_perm(w[2 * i], w[2 * i + 1], h ? 0x7632u : 0x5410u);  // rows 4h .. 4h+3
-            const uint32_t y = z >> 8;
-            d[i][4 * h] = int4::low_pair<DT>(z);
-            d[i][4 * h + 1] = int4::high_pair<DT>(z);
-            d[i][4 * h + 2] = int4::low_pair<DT>(y);
-            d[i][4 * h + 3] = int4::high_pair<DT>(y);
+// a ring's slot and the parity of its current pass
+template <int R>
+struct Ring {
+    int i = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void advance(int by = 1) {
+        i += by;
+        if (i >= R) {
+            i -= R;
+            parity ^= 1u;
         }
     }
+};
+
+// One lane of a converged warp.  A branch on elect.sync tells the compiler that a single lane
+// runs it: under `lane == 0` it wraps every tcgen05 instruction, whose operands are uniform
+// registers, in a loop over the lanes, ~100 cycles each.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
+}
+
+template <int R>
+__device__ __forceinline__ void regs_inc() {
+    if constexpr (R > 0) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(R));
+}
+template <int R>
+__device__ __forceinline__ void regs_dec() {
+    if constexpr (R > 0) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(R));
+}
+
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &lo, float &hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// Column of the tile that row r of the M operand holds: a core matrix's 8 rows are 4 columns
+// of the tile's left half and 4 of its right half, so that a decode lane's two 16-byte reads
+// of words are both conflict-free.
+__device__ __forceinline__ int column_of(int r) { return 4 * (r >> 3) + (r & 3) + ((r & 4) << 4); }
+
+// K rows 4h .. 4h+3 of the core matrix of 8 words (w0: columns 0-3, w1: 4-7): two columns'
+// halves side by side decode together
+template <class DT>
+__device__ __forceinline__ void decode_half(const uint4 w0, const uint4 w1, int h, uint4 (&out)[4]) {
+    const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+    uint32_t d[4][4];
 #pragma unroll
-    for (int r = 0; r < 8; ++r) out[r] = make_uint4(d[0][r], d[1][r], d[2][r], d[3][r]);
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t z = __byte_perm(w[2 * i], w[2 * i + 1], h ? 0x7632u : 0x5410u);
+        const uint32_t y = z >> 8;
+        d[i][0] = int4::low_pair<DT>(z);
+        d[i][1] = int4::high_pair<DT>(z);
+        d[i][2] = int4::low_pair<DT>(y);
+        d[i][3] = int4::high_pair<DT>(y);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) out[r] = make_uint4(d[0][r], d[1][r], d[2][r], d[3][r]);
 }
 
 __device__ __forceinline__ float ld_dsmem_f32(uint32_t local_addr, uint32_t rank) {
@@ -112,63 +192,71 @@ __device__ __forceinline__ float ld_dsmem_f32(uint32_t local_addr, uint32_t rank
     return v;
 }
 
-// element (m, n) through the epilogue
+// element i = m * N + n, e = its epilogue operand
 template <class DT, int POSTOP, bool OUT_F32>
-__device__ __forceinline__ void store(const Params &p, int m, int n, float v) {
-    const size_t i = (size_t)m * p.N + n;
-    v = epi<POSTOP, OUT_F32>(v, epi_in<DT, POSTOP, OUT_F32>(p.Other, p.Bias, i, n));
+__device__ __forceinline__ void store(const Params &p, size_t i, float v, float e) {
+    v = epi<POSTOP, OUT_F32>(v, e);
     if constexpr (OUT_F32) reinterpret_cast<float *>(p.C)[i] = v;
     else reinterpret_cast<uint16_t *>(p.C)[i] = DT::fromf(v);
 }
 
-template <int MT, class DT, int POSTOP, bool OUT_F32>
-__global__ void __launch_bounds__(Cfg<MT>::kThreads, Cfg<MT>::kCtasPerSm)
-    gemm_int4_kernel(const Params p, const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB) {
-    using C = Cfg<MT>;
-    extern __shared__ __align__(1024) char smem_raw[];
-    char *smem = smem_raw + ((1024u - (tc::smem_addr(smem_raw) & 1023u)) & 1023u);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int n0 = blockIdx.x * BN;
-    const int G = p.K / kGS;
-    int m0 = blockIdx.y * MT, m_end = p.M, expert = 0;
+struct Tile {
+    int n0, m0, rows, expert;
+};
+
+// tile t: row tile t / strips, column strip t % strips (neighbours share their rows)
+template <int MT>
+__device__ __forceinline__ Tile tile_of(const Params &p, const int *first, int t) {
+    const int r = t / p.strips;
+    Tile ti;
+    ti.n0 = (t - r * p.strips) * BN;
+    ti.expert = 0;
+    ti.m0 = r * MT;
+    int end = p.M;
     if (p.meta) {
-        // the expert of this 128-row tile: the last one whose first tile is <= it
-        pdl_wait();
-        constexpr int kSub = MT < kMetaTile ? kMetaTile / MT : 1;
-        const int tile = blockIdx.y / kSub, E = p.E;
-        if (tile >= p.meta[2 * E + 1]) return;
-        int lo = 0, hi = E - 1;
+        int lo = 0, hi = p.E - 1;  // the last expert whose first tile is <= r
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (p.meta[E + 1 + mid] <= tile) lo = mid;
+            if (first[mid] <= r) lo = mid;
             else hi = mid - 1;
         }
-        expert = lo;
-        m0 = p.meta[lo] + (tile - p.meta[E + 1 + lo]) * kMetaTile + (blockIdx.y % kSub) * MT;
-        m_end = p.meta[lo + 1];
-        if (m0 >= m_end) return;
+        ti.expert = lo;
+        const int row0 = min(max(p.meta[lo], 0), p.M);
+        end = min(max(p.meta[lo + 1], row0), p.M);
+        ti.m0 = row0 + (r - first[lo]) * MT;
     }
-    const int rows = min(MT, m_end - m0);
-    const int g0 = (int)((long long)G * blockIdx.z / p.SK), g1 = (int)((long long)G * (blockIdx.z + 1) / p.SK);
-    const int ng = g1 - g0;
+    ti.rows = min(MT, end - ti.m0);
+    return ti;
+}
 
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::bars);
-    uint64_t *load_empty = full + C::kLoads;
-    uint64_t *dec_full = load_empty + C::kLoads;
-    uint64_t *dec_empty = dec_full + C::kDecs;
-    uint64_t *acc_full = dec_empty + C::kDecs;
+template <int MT, class DT, int POSTOP, bool OUT_F32>
+__global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
+    gemm_int4_kernel(const Params p, const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB) {
+    using C = Plan<MT>;
+    extern __shared__ __align__(1024) char smem_raw[];
+    char *smem = smem_raw + ((1024u - (tc::smem_addr(smem_raw) & 1023u)) & 1023u);
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const int G = p.K / kGS;
+    const int sk = blockIdx.x % p.SK;
+    const int g0 = (int)((long long)G * sk / p.SK), ng = (int)((long long)G * (sk + 1) / p.SK) - g0;
+
+    uint64_t *ready = reinterpret_cast<uint64_t *>(smem + C::bars);  // a step's operands are in place
+    uint64_t *done = ready + C::kSteps;                              // its MMAs have read them
+    uint64_t *words_full = done + C::kSteps;
+    uint64_t *words_empty = words_full + C::kWords;
+    uint64_t *acc_full = words_empty + C::kWords;
     uint64_t *acc_empty = acc_full + C::kAccBufs;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + C::kAccBufs);
-    static_assert((2 * C::kLoads + 2 * C::kDecs + 2 * C::kAccBufs) * 8 + 4 <= 256, "barriers");
+    int *first = reinterpret_cast<int *>(smem + C::first);
 
     if (tid == 0) {
-        for (int s = 0; s < C::kLoads; ++s) {
-            tc::mbar_init(&full[s], 1);
-            tc::mbar_init(&load_empty[s], 1 + 8);  // the MMAs, and 4 decode warps for each half
+        for (int s = 0; s < C::kSteps; ++s) {
+            tc::mbar_init(&ready[s], 1 + 4);  // the activations' producer and the decode team's warps
+            tc::mbar_init(&done[s], 1);
         }
-        for (int d = 0; d < C::kDecs; ++d) {
-            tc::mbar_init(&dec_full[d], 4);
-            tc::mbar_init(&dec_empty[d], 1);
+        for (int s = 0; s < C::kWords; ++s) {
+            tc::mbar_init(&words_full[s], 1);
+            tc::mbar_init(&words_empty[s], 4);
         }
         for (int b = 0; b < C::kAccBufs; ++b) {
             tc::mbar_init(&acc_full[b], 1);
@@ -176,194 +264,337 @@ __global__ void __launch_bounds__(Cfg<MT>::kThreads, Cfg<MT>::kCtasPerSm)
         }
         tc::fence_mbar_init();
     }
-    if (warp == 1) tc::tmem_alloc(tmem_slot, C::kTmemCols);
+    if (warp == 3) tc::tmem_alloc(tmem_slot, C::kTmemCols);
+    if (p.meta) {
+        pdl_wait();  // meta comes from the routing kernel
+        if (warp == 0) {
+            int sum = 0;
+            for (int e0 = 0; e0 < p.E; e0 += 32) {
+                const int e = e0 + lane;
+                int x = 0;
+                if (e < p.E) {
+                    const int lo = min(max(p.meta[e], 0), p.M), hi = min(max(p.meta[e + 1], lo), p.M);
+                    x = (hi - lo + MT - 1) / MT;
+                }
+                int incl = x;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int y = __shfl_up_sync(0xffffffffu, incl, o);
+                    if (lane >= o) incl += y;
+                }
+                if (e < p.E) first[e] = sum + incl - x;
+                sum += __shfl_sync(0xffffffffu, incl, 31);
+            }
+            if (lane == 0) first[p.E] = sum;
+        }
+    }
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = *tmem_slot;
+    const int ntiles = (p.meta ? first[p.E] : (p.M + MT - 1) / MT) * p.strips;
+    const int t0 = blockIdx.x / p.SK, tstep = gridDim.x / p.SK;
 
-    // promotion threads: column n (TMEM lane) and rows jbase .. jbase + kCols - 1 of the tile
-    const int pw = warp - (2 + 4 * C::NT);
+    // promotion threads: row r of the M operand (a column of C) and the tile's activation rows
+    // jbase .. jbase + kCols - 1
+    const int pw = warp - (4 + 4 * C::NT);
     const int quad = warp & 3;
-    const int jbase = pw >= 4 ? C::kCols : 0;
-    const int n = n0 + 32 * quad + lane;
-    float acc[C::kCols];
+    const int jbase = (pw >> 2) * C::kCols;
+    const int col = column_of(32 * quad + lane);
 
-    if (warp == 0) {
-        // ---------------- producer ----------------
-        if (lane == 0) {
-            if (!p.meta) pdl_wait();
-            int issued = 0;
-            for (int i = 0; i < ng; ++i) {
-                const int s = i % C::kLoads;
-                if (i >= C::kLoads && !tc::mbar_wait(&load_empty[s], ((i / C::kLoads) - 1) & 1)) break;
-                tc::mbar_expect_tx(&full[s], C::kABytes + kPackBytes);
-                const int grp = g0 + i;
-                tc::tma_load_2d(smem + C::pack + s * kPackBytes, &tmB, n0,
-                                expert * (p.K / int4::kRowsPerWord) + grp * int4::kWordsPerGroup, &full[s]);
-                char *a = smem + C::a + s * C::kABytes;
-                tc::tma_load_2d(a, &tmA, grp * kGS, m0, &full[s]);
-                tc::tma_load_2d(a + C::kABytes / 2, &tmA, grp * kGS + kHalf, m0, &full[s]);
-                ++issued;
-            }
-            // copies still in flight must land before the block can exit
-            for (int i = issued < C::kLoads ? 0 : issued - C::kLoads; i < issued; ++i)
-                tc::mbar_wait(&full[i % C::kLoads], (i / C::kLoads) & 1);
-        }
-    } else if (warp == 1) {
-        // ---------------- MMA issuer ----------------
-        if (lane == 0) {
-            // M operand MN-major (bit 15), N operand K-major
-            const uint32_t idesc = tc::idesc_f16(DT::kBF16, BN, (rows + 15) & ~15) | (1u << 15);
+    if (warp < 4) {
+        regs_dec<C::kRegsOther>();
+        if (warp == 0) {
+            // ---------------- activations ----------------
+            pdl_wait();
+            Ring<C::kSteps> q;
             bool ok = true;
-            for (int i = 0; i < ng && ok; ++i) {
-                const int s = i % C::kLoads, b = i % C::kAccBufs;
-                if (!tc::mbar_wait(&full[s], (i / C::kLoads) & 1)) break;
-                if (i >= C::kAccBufs && !tc::mbar_wait(&acc_empty[b], ((i / C::kAccBufs) - 1) & 1)) break;
-                const uint32_t act = tc::smem_addr(smem + C::a + s * C::kABytes);
-#pragma unroll 1
-                for (int h = 0; h < 2; ++h) {
-                    const int x = 2 * i + h, d = x % C::kDecs;
-                    if (!tc::mbar_wait(&dec_full[d], (x / C::kDecs) & 1)) {
+            for (int t = t0; t < ntiles && ok; t += tstep) {
+                const Tile ti = tile_of<MT>(p, first, t);
+                const int boxes = (ti.rows + C::kBoxRows - 1) / C::kBoxRows;
+                for (int x = 0; x < 2 * ng; ++x, q.advance()) {
+                    if (!tc::mbar_wait(&done[q.i], q.parity ^ 1u)) {
+                        ok = false;
+                        break;
+                    }
+                    if (elect_one()) {
+                        tc::mbar_expect_tx(&ready[q.i], boxes * C::kBoxBytes);
+                        char *a = smem + C::a + q.i * C::kABytes;
+                        for (int b = 0; b < boxes; ++b)
+                            tc::tma_load_2d(a + b * C::kBoxBytes, &tmA, g0 * kGS + x * kStepK,
+                                            ti.m0 + b * C::kBoxRows, &ready[q.i]);
+                    }
+                    __syncwarp();
+                }
+            }
+            if (!ok) {  // copies still in flight must land before the block can exit
+                for (int s = 0; s < C::kSteps; ++s) {
+                    q.advance();
+                    tc::mbar_wait(&ready[q.i], q.parity ^ 1u);
+                }
+            }
+        } else if (warp == 1) {
+            // ---------------- MMA issuer ----------------
+            Ring<C::kSteps> q;
+            Ring<C::kAccBufs> b;
+            bool ok = true;
+            for (int t = t0; t < ntiles && ok; t += tstep) {
+                const Tile ti = tile_of<MT>(p, first, t);
+                // M operand MN-major (bit 15), N operand K-major
+                const uint32_t idesc = tc::idesc_f16(DT::kBF16, BN, (ti.rows + 15) & ~15) | (1u << 15);
+                for (int x = 0; x < 2 * ng; ++x, q.advance()) {
+                    if (!(x & 1) && !tc::mbar_wait(&acc_empty[b.i], b.parity ^ 1u)) {
+                        ok = false;
+                        break;
+                    }
+                    if (!tc::mbar_wait(&ready[q.i], q.parity)) {
                         ok = false;
                         break;
                     }
                     tc::fence_after_sync();
-                    const uint32_t w = tc::smem_addr(smem + C::dec + d * kDecStageBytes);
+                    const uint64_t w = tc::sdesc_kmajor_noswz(tc::smem_addr(smem + C::dec + q.i * kDecBytes), kDecLBO,
+                                                              kDecSBO);
+                    const uint64_t v = tc::sdesc_kmajor_sw128(tc::smem_addr(smem + C::a + q.i * C::kABytes));
+                    if (elect_one()) {
+                        // (addresses stay below 2^18: a step along K adds to the address field only)
 #pragma unroll
-                    for (int kk = 0; kk < kHalf / 16; ++kk)
-                        tc::mma_ss_f16(tmem + b * MT, tc::sdesc_kmajor_noswz(w + kk * 2 * kDecLBO, kDecLBO, kDecSBO),
-                                       tc::sdesc_kmajor_sw128(act + h * (C::kABytes / 2) + kk * 32), idesc,
-                                       (h | kk) != 0);
-                    tc::mma_commit(&dec_empty[d]);
+                        for (int kk = 0; kk < kStepK / 16; ++kk)
+                            tc::mma_ss_f16(tmem + b.i * MT, w + (uint64_t)(kk * 2 * kDecLBO / 16),
+                                           v + (uint64_t)(kk * 2), idesc, ((x & 1) | kk) != 0);
+                        tc::mma_commit(&done[q.i]);
+                        if (x & 1) tc::mma_commit(&acc_full[b.i]);
+                    }
+                    __syncwarp();
+                    if (x & 1) b.advance();
                 }
-                if (!ok) break;
-                tc::mma_commit(&load_empty[s]);
-                tc::mma_commit(&acc_full[b]);
+            }
+        } else if (warp == 2) {
+            // ---------------- packed words (weights: read before the previous kernel ends) ----------------
+            Ring<C::kWords> q;
+            bool ok = true;
+            for (int t = t0; t < ntiles && ok; t += tstep) {
+                const Tile ti = tile_of<MT>(p, first, t);
+                const int row0 = (ti.expert * G + g0) * int4::kWordsPerGroup;
+                for (int x = 0; x < 2 * ng; ++x, q.advance()) {
+                    if (!tc::mbar_wait(&words_empty[q.i], q.parity ^ 1u)) {
+                        ok = false;
+                        break;
+                    }
+                    if (elect_one()) {
+                        tc::mbar_expect_tx(&words_full[q.i], kWordBytes);
+                        tc::tma_load_2d(smem + C::words + q.i * kWordBytes, &tmB, ti.n0,
+                                        row0 + x * (kStepK / int4::kRowsPerWord), &words_full[q.i]);
+                    }
+                    __syncwarp();
+                }
+            }
+            if (!ok) {
+                for (int s = 0; s < C::kWords; ++s) {
+                    q.advance();
+                    tc::mbar_wait(&words_full[q.i], q.parity ^ 1u);
+                }
             }
         }
-    } else if (warp < 2 + 4 * C::NT) {
+    } else if (warp < 4 + 4 * C::NT) {
         // ---------------- decode ----------------
-        const int team = (warp - 2) >> 2;
-        const int task = ((warp - 2) & 3) * 32 + lane;  // 8 word rows x 16 column blocks
+        regs_dec<C::kRegsOther>();
+        const int team = (warp - 4) >> 2;
+        const int task = ((warp - 4) & 3) * 32 + lane;  // 8 word rows x 16 column blocks
         const int wr = task >> 4, nb = task & 15;
-        // two 16-byte chunks per lane, read in the other order by every second four lanes, so
-        // that both reads of a quarter-warp touch 8 distinct 16-byte bank groups
-        const int sw = (nb >> 2) & 1;
-        for (int x = team; x < 2 * ng; x += C::NT) {
-            const int i = x >> 1, s = i % C::kLoads, d = x % C::kDecs;
-            if (!tc::mbar_wait(&full[s], (i / C::kLoads) & 1)) break;
-            const uint4 *src = reinterpret_cast<const uint4 *>(smem + C::pack + s * kPackBytes +
-                                                               ((x & 1) * 8 + wr) * (BN * 4) + nb * 32);
-            const uint4 c0 = src[sw], c1 = src[sw ^ 1];
-            uint4 out[8];
-            decode8<DT>(sw ? c1 : c0, sw ? c0 : c1, out);
-            if (x >= C::kDecs && !tc::mbar_wait(&dec_empty[d], ((x / C::kDecs) - 1) & 1)) break;
-            char *dst = smem + C::dec + d * kDecStageBytes + nb * kDecSBO + wr * 128;
+        const char *src0 = smem + C::words + wr * (BN * 4) + nb * 16;
+        char *dst0 = smem + C::dec + nb * kDecSBO + wr * 128;
+        Ring<C::kWords> qw;
+        Ring<C::kSteps> q;
+        qw.advance(team);
+        q.advance(team);
+        bool ok = true;
+        int x = team;  // steps over all tiles; each team takes every NT-th
+        for (int t = t0; t < ntiles && ok; t += tstep) {
+            for (; x < 2 * ng; x += C::NT, qw.advance(C::NT), q.advance(C::NT)) {
+                if (!tc::mbar_wait(&words_full[qw.i], qw.parity)) {
+                    ok = false;
+                    break;
+                }
+                const char *src = src0 + qw.i * kWordBytes;
+                const uint4 w0 = *reinterpret_cast<const uint4 *>(src);
+                const uint4 w1 = *reinterpret_cast<const uint4 *>(src + 256);
+                uint4 out[4];
+                decode_half<DT>(w0, w1, 0, out);
+                if (!tc::mbar_wait(&done[q.i], q.parity ^ 1u)) {
+                    ok = false;
+                    break;
+                }
+                char *dst = dst0 + q.i * kDecBytes;
 #pragma unroll
-            for (int r = 0; r < 8; ++r) *reinterpret_cast<uint4 *>(dst + r * 16) = out[r];
-            tc::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                tc::mbar_arrive(&dec_full[d]);
-                tc::mbar_arrive(&load_empty[s]);
+                for (int r = 0; r < 4; ++r) *reinterpret_cast<uint4 *>(dst + r * 16) = out[r];
+                decode_half<DT>(w0, w1, 1, out);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) *reinterpret_cast<uint4 *>(dst + 64 + r * 16) = out[r];
+                tc::fence_proxy_async_smem();
+                __syncwarp();
+                if (elect_one()) {
+                    tc::mbar_arrive(&ready[q.i]);
+                    tc::mbar_arrive(&words_empty[qw.i]);
+                }
+                __syncwarp();
             }
+            x -= 2 * ng;
         }
     } else {
-        // ---------------- promotion ----------------
+        // ---------------- promotion and epilogue ----------------
+        regs_inc<C::kRegsPromote>();
+        // the scales of the next kAhead groups are on their way, as loaded: converting or moving
+        // one before its group would wait for it
+        constexpr int kAhead = 4;
+        constexpr int kLd = MT == 32 ? 16 : 32;  // accumulator columns per round of loads
+        uint16_t sc[kAhead];
+        const uint16_t *sp = nullptr;
+        auto scales_of = [&](int t) {
+            const Tile ti = tile_of<MT>(p, first, t);
+            const int n = ti.n0 + col;
+            sp = p.S + ((size_t)ti.expert * G + g0) * p.N + (n < p.N ? n : 0);
 #pragma unroll
-        for (int j = 0; j < C::kCols; ++j) acc[j] = 0.0f;
-        const bool nok = n < p.N;
-        const uint16_t *sp = p.S + ((size_t)expert * G + g0) * p.N + (nok ? n : 0);
-        constexpr int kAhead = 4;  // scales are requested this many groups early
-        float sc[kAhead];
+            for (int k = 0; k < kAhead; ++k) sc[k] = __ldg(sp + (size_t)min(k, ng - 1) * p.N);
+        };
+        if (t0 < ntiles) scales_of(t0);
+        Ring<C::kAccBufs> b;
+        bool ok = true;
+        for (int t = t0; t < ntiles && ok; t += tstep) {
+            const Tile ti = tile_of<MT>(p, first, t);
+            const int n = ti.n0 + col;
+            uint64_t acc[C::kCols / 2];
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) sc[k] = k < ng ? DT::tof(__ldg(sp + (size_t)k * p.N)) : 0.0f;
-        for (int i = 0; i < ng; ++i) {
-            const int b = i % C::kAccBufs;
-            const float s = sc[0];
+            for (int j = 0; j < C::kCols / 2; ++j) acc[j] = 0ull;
+            for (int i0 = 0; i0 < ng && ok; i0 += kAhead) {
 #pragma unroll
-            for (int k = 0; k + 1 < kAhead; ++k) sc[k] = sc[k + 1];
-            sc[kAhead - 1] = i + kAhead < ng ? DT::tof(__ldg(sp + (size_t)(i + kAhead) * p.N)) : 0.0f;
-            if (!tc::mbar_wait(&acc_full[b], (i / C::kAccBufs) & 1)) break;
-            tc::fence_after_sync();
-            const uint32_t taddr = tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(b * MT + jbase);
+                for (int k = 0; k < kAhead; ++k) {
+                    const int i = i0 + k;
+                    if (i >= ng) break;
+                    if (!tc::mbar_wait(&acc_full[b.i], b.parity)) {
+                        ok = false;
+                        break;
+                    }
+                    tc::fence_after_sync();
+                    const float s1 = DT::tof(sc[k]);
+                    const uint64_t s = pack2(s1, s1);
+                    sc[k] = __ldg(sp + (size_t)min(i + kAhead, ng - 1) * p.N);
+                    const uint32_t taddr = tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(b.i * MT + jbase);
 #pragma unroll
-            for (int c = 0; c < C::kCols; c += 16) {
-                if (jbase + c < rows) {  // warp-uniform
-                    float v[16];
-                    tc::tmem_ld<16>(taddr + c, v);
-                    tc::tmem_wait_ld();
+                    for (int c = 0; c < C::kCols; c += kLd) {
+                        if (jbase + c < ti.rows) {  // warp-uniform
+                            float v[kLd];
+                            tc::tmem_ld<16>(taddr + c, *reinterpret_cast<float(*)[16]>(&v[0]));
+                            if constexpr (kLd == 32)
+                                tc::tmem_ld<16>(taddr + c + 16, *reinterpret_cast<float(*)[16]>(&v[16]));
+                            tc::tmem_wait_ld();
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) acc[c + j] = fmaf(v[j], s, acc[c + j]);
+                            for (int j = 0; j < kLd; j += 2)
+                                acc[(c + j) / 2] = fma2(pack2(v[j], v[j + 1]), s, acc[(c + j) / 2]);
+                        }
+                    }
+                    tc::fence_before_sync();
+                    __syncwarp();
+                    if (elect_one()) tc::mbar_arrive(&acc_empty[b.i]);
+                    __syncwarp();
+                    b.advance();
                 }
             }
-            tc::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&acc_empty[b]);
-        }
-        if (p.SK == 1) {
-            pdl_wait();
-            if (nok) {
+            if (p.SK > 1) {
+                // one tile: its sums [rows][128] go into the stages, whose last readers (the MMAs of the
+                // last group) are through, and are joined below
+                float *part = reinterpret_cast<float *>(smem);
 #pragma unroll
-                for (int j = 0; j < C::kCols; ++j)
-                    if (jbase + j < rows) store<DT, POSTOP, OUT_F32>(p, m0 + jbase + j, n, acc[j]);
+                for (int j = 0; j < C::kCols; j += 2) {
+                    float v0, v1;
+                    unpack2(acc[j / 2], v0, v1);
+                    part[(jbase + j) * BN + col] = v0;
+                    part[(jbase + j + 1) * BN + col] = v1;
+                }
+                break;
             }
-            pdl_launch_dependents();
+            if (t + tstep < ntiles) scales_of(t + tstep);
+            pdl_wait();
+            if (n < p.N) {
+                constexpr int kBatch = MT == 32 ? 8 : 16;  // rows whose epilogue operands are in flight together
+                const size_t i0 = (size_t)(ti.m0 + jbase) * p.N + n;
+#pragma unroll
+                for (int c = 0; c < C::kCols; c += kBatch) {
+                    float e[kBatch];
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j)
+                        e[j] = (POSTOP == 1 || POSTOP == 2) && jbase + c + j >= ti.rows
+                                   ? 0.0f
+                                   : epi_in<DT, POSTOP, OUT_F32>(p.Other, p.Bias, i0 + (size_t)(c + j) * p.N, n);
+#pragma unroll
+                    for (int j = 0; j < kBatch; j += 2) {
+                        float v0, v1;
+                        unpack2(acc[(c + j) / 2], v0, v1);
+                        const size_t i = i0 + (size_t)(c + j) * p.N;
+                        if (jbase + c + j < ti.rows) store<DT, POSTOP, OUT_F32>(p, i, v0, e[j]);
+                        if (jbase + c + j + 1 < ti.rows) store<DT, POSTOP, OUT_F32>(p, i + p.N, v1, e[j + 1]);
+                    }
+                }
+            }
         }
+        pdl_launch_dependents();
+        regs_dec<C::kRegsOther>();  // every warp goes on with the same share
     }
     if (p.SK > 1) {
-        // the split's sums [rows][128] in the stages, which the MMAs have finished reading
+        const Tile ti = tile_of<MT>(p, first, t0);
+        const float *part = reinterpret_cast<const float *>(smem);
         __syncthreads();
-        float *part = reinterpret_cast<float *>(smem);
-        if (warp >= 2 + 4 * C::NT) {
-#pragma unroll
-            for (int j = 0; j < C::kCols; ++j)
-                if (jbase + j < rows) part[(jbase + j) * BN + 32 * quad + lane] = acc[j];
-        }
         gemv::cluster_sync_all();
         pdl_wait();
-        const int r0 = rows * (int)blockIdx.z / p.SK, r1 = rows * ((int)blockIdx.z + 1) / p.SK;
+        const int r0 = ti.rows * sk / p.SK, r1 = ti.rows * (sk + 1) / p.SK;
         for (int x = r0 * BN + tid; x < r1 * BN; x += C::kThreads) {
             const uint32_t la = tc::smem_addr(part + x);
             float v = 0.0f;
             for (int r = 0; r < p.SK; ++r) v += ld_dsmem_f32(la, (uint32_t)r);
-            if (n0 + x % BN < p.N) store<DT, POSTOP, OUT_F32>(p, m0 + x / BN, n0 + x % BN, v);
+            const int n = ti.n0 + x % BN;
+            const size_t i = (size_t)(ti.m0 + x / BN) * p.N + n;
+            if (n < p.N) store<DT, POSTOP, OUT_F32>(p, i, v, epi_in<DT, POSTOP, OUT_F32>(p.Other, p.Bias, i, n));
         }
-        pdl_launch_dependents();
         gemv::cluster_sync_all();  // every CTA's sums stay until all have read them
     }
     tc::fence_before_sync();
     __syncthreads();
-    if (warp == 1) {
+    if (warp == 3) {
         tc::fence_after_sync();
         tc::tmem_dealloc(tmem, C::kTmemCols);
     }
 }
 
 template <int MT>
-cudaError_t launch(const GemvArgs &a, const int *meta, int E) {
-    using C = Cfg<MT>;
+cudaError_t launch(const GemvArgs &a, int sms, const int *meta, int E) {
+    using C = Plan<MT>;
     CUtensorMap mapA, mapB;
     cudaError_t e = tc::make_map_sw128(
         &mapA, a.A, a.dtype == TERNOCL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-        a.M, a.K, MT);
+        a.M, a.K, C::kBoxRows);
     if (e != cudaSuccess) return e;
     e = tc::make_map_plain(&mapB, a.B, CU_TENSOR_MAP_DATA_TYPE_INT32, 4, (meta ? E : 1) * (a.K / int4::kRowsPerWord),
-                           a.N, int4::kWordsPerGroup, BN);
+                           a.N, kStepK / int4::kRowsPerWord, BN);
     if (e != cudaSuccess) return e;
-    const Params p{(const uint16_t *)a.S, a.C, (const uint16_t *)a.Other, a.Bias, a.M, a.N, a.K, a.SK, meta, E};
+    const int strips = (a.N + BN - 1) / BN;
+    const Params p{(const uint16_t *)a.S, a.C, (const uint16_t *)a.Other, a.Bias, a.M, a.N, a.K, a.SK, strips, meta, E};
+    // grouped: an upper bound, every expert adds at most one partial tile
+    const long long tiles = ((long long)(a.M + MT - 1) / MT + (meta ? E : 0)) * strips;
+    const long long slots = (long long)sms * C::kCtasPerSm;
+    const int grid = a.SK > 1 ? (int)tiles * a.SK : (int)(tiles < slots ? tiles : slots);
     return dispatch_epilogue<GemvArgs>(a, [&](auto dt, auto po, auto of) -> cudaError_t {
         using DT = typename decltype(dt)::type;
         auto kern = gemm_int4_kernel<MT, DT, decltype(po)::value, decltype(of)::value>;
+        if (C::kRegsPromote > 0 && !smem_attr_known((const void *)kern, C::total)) {
+            // the register shares are drawn from what the block launches with
+            cudaFuncAttributes fa;
+            const cudaError_t fe = cudaFuncGetAttributes(&fa, kern);
+            if (fe != cudaSuccess) return fe;
+            if (fa.numRegs != C::kLaunchRegs) return cudaErrorInvalidConfiguration;
+        }
         cudaError_t err = ensure_smem(kern, C::total);
         if (err != cudaSuccess) return err;
-        const int strips = (a.N + BN - 1) / BN;
-        // grouped: every expert adds at most one partial 128-row tile
-        const int tiles = meta ? ((a.M + kMetaTile - 1) / kMetaTile + E) * (MT < kMetaTile ? kMetaTile / MT : 1)
-                               : (a.M + MT - 1) / MT;
-        return launch_kernel_cluster(kern, dim3(strips, tiles, a.SK), dim3(C::kThreads), (size_t)C::total, a.stream,
-                                     dim3(1, 1, a.SK), p, mapA, mapB);
+        return launch_kernel_cluster(kern, dim3(grid), dim3(C::kThreads), (size_t)C::total, a.stream, dim3(a.SK, 1, 1),
+                                     p, mapA, mapB);
     });
 }
 
@@ -371,17 +602,19 @@ cudaError_t launch(const GemvArgs &a, const int *meta, int E) {
 
 cudaError_t int4_gemm_launch(const GemvArgs &a, int sms, const int *meta, int E) {
     GemvArgs b = a;
-    // activation rows per CTA: what the rows (grouped: an expert's average) fill
+    // activation rows per tile: what the rows (grouped: an expert's average) fill
     const long long per = meta ? (a.M + E - 1) / E : a.M;
-    const int MT = per <= 32 ? 32 : per <= 64 ? 64 : 128;
+    const int MT = per <= 32 ? 32 : per <= 64 ? 64 : per <= 128 ? 128 : 256;
     // K split over a cluster while the tiles leave SMs without work
     const long long tiles = (long long)((a.N + gemm4::BN - 1) / gemm4::BN) * ((a.M + MT - 1) / MT);
     int sk = 1;
     if (!meta)
         while (sk < 8 && 2 * sk <= a.K / kGS && tiles * 2 * sk <= sms) sk *= 2;
     b.SK = sk;
-    return MT == 32 ? gemm4::launch<32>(b, meta, E) : MT == 64 ? gemm4::launch<64>(b, meta, E)
-                                                               : gemm4::launch<128>(b, meta, E);
+    return MT == 32    ? gemm4::launch<32>(b, sms, meta, E)
+           : MT == 64  ? gemm4::launch<64>(b, sms, meta, E)
+           : MT == 128 ? gemm4::launch<128>(b, sms, meta, E)
+                       : gemm4::launch<256>(b, sms, meta, E);
 }
 
 cudaError_t read_device_error_gemm_int4(unsigned *out, int reset) { return tc::read_tu_error(out, reset); }
