@@ -355,7 +355,7 @@ int ternocl_moe_decode_down_sum(const int32_t *ids, const void *H, const void *R
  *
  * Linear layer:  C[m,n] = DT(epi( sum_k A[m,k] * code(B[k,n]) * S[k/128, n] )).
  * algo: GEMV (decode), GEMM (tcgen05), or AUTO (the GEMV up to M = 8).  No workspace: a K
- * split stays within one thread-block cluster.  M <= 524280. */
+ * split stays within one thread-block cluster.  M <= 524280; C and Other 16-byte aligned. */
 int ternocl_int4_upcvt(const void *A, const uint32_t *B, const void *S, void *C, const void *Other,
                        const void *Bias, int M, int N, int K, int dtype, int postop, int out_f32, int algo,
                        void *stream);
@@ -363,7 +363,7 @@ int ternocl_int4_upcvt(const void *A, const uint32_t *B, const void *S, void *C,
 /* Grouped GEMM of MoE prefill with 4-bit experts, as ternocl_moe_gemm: for the rows p of
  * every expert e (meta of ternocl_moe_route), C[p, n] = epi(A[p] . B_e[:, n]); B_all
  * [E, K/8, N], S_all [E, K/128, N]; Other_all [G, N] (POSTOP 1/2); no bias.  Rows of C that
- * belong to no expert are not written.  G <= 2^20. */
+ * belong to no expert are not written.  G <= 2^20; C_all and Other_all 16-byte aligned. */
 int ternocl_moe_gemm_int4(const int32_t *meta, const void *A_all, const uint32_t *B_all, const void *S_all,
                           void *C_all, const void *Other_all, int G, int N, int K, int num_experts, int dtype,
                           int postop, int out_f32, void *stream);

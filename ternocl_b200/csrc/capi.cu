@@ -766,6 +766,7 @@ int ternocl_int4_upcvt(const void *A, const uint32_t *B, const void *S, void *C,
     if (st != TERNOCL_OK) return st;
     if (algo < TERNOCL_ALGO_AUTO || algo > TERNOCL_ALGO_GEMM) return TERNOCL_ERR_ARG;
     if (M > kMaxGridYZ) return TERNOCL_ERR_SHAPE;
+    if (!aligned(C, 16) || (Other && !aligned(Other, 16))) return TERNOCL_ERR_ARG;  // 16-byte stores and loads
     if (M == 0) return TERNOCL_OK;
     GemvArgs a;
     a.A = A; a.B = B; a.S = S; a.C = C; a.Other = Other; a.Bias = Bias;
@@ -793,6 +794,7 @@ int ternocl_moe_gemm_int4(const int32_t *meta, const void *A_all, const uint32_t
     if (st != TERNOCL_OK) return st;
     if (postop == TERNOCL_POSTOP_BIAS) return TERNOCL_ERR_ARG;
     if (!meta || num_experts < 1 || num_experts > 1024) return TERNOCL_ERR_ARG;
+    if (!aligned(C_all, 16) || (Other_all && !aligned(Other_all, 16))) return TERNOCL_ERR_ARG;
     // the weights' rows are one tensor map's (32-bit coordinates), the row tiles a grid's
     if ((long long)num_experts * (K / 8) > 0x7fffffffLL || G > (1 << 20)) return TERNOCL_ERR_SHAPE;
     if (G == 0) return TERNOCL_OK;

@@ -12,10 +12,13 @@
 // operand (up to MT): then a TMEM lane is a column n, a thread scales its whole lane by one
 // S[g,n], and the N extent follows the rows that are there.
 //
-// Persistent CTAs walk tiles of 128 columns x MT rows; a step is half a group (K = 64):
+// Persistent CTAs walk tiles of 128 columns x MT rows; a step is half a group (K = 64).  At
+// MT = 256 two CTAs of a cluster work as a pair on 256 columns x 256 rows (cta_group::2):
+// each holds its own columns' weights and half of the rows' activations, and every MMA
+// reads both halves, so the activations cross from L2 once for 256 columns.  Roles:
 //   warp 0      the activations of a step: TMA boxes of 64 rows x 64 (128-byte swizzle);
-//   warp 1      the MMA issuer: per step 4 tcgen05.mma kind::f16 (M=128, N=rows rounded up to
-//               16, K=16) into one of kAccBufs accumulators;
+//   warp 1      the MMA issuer (of a pair: the first CTA's): per step 4 tcgen05.mma kind::f16
+//               (M=128 a CTA, N=rows rounded up, K=16) into one of kAccBufs accumulators;
 //   warp 2      the packed words of a step: one TMA box of 8 word rows x 128 columns;
 //   warp 3      TMEM allocation;
 //   4 NT warps  decode, NT teams of 4 that take the steps in turn: one lane makes one 8 x 8 core
@@ -26,8 +29,9 @@
 // and each adds up a share of the rows in split order over distributed shared memory.
 //
 // What bounds it: for many rows the MMAs (1024 cycles for a group at MT = 256) and, close
-// behind, the issue slots of decode and promotion; for few rows the decode, which all 16 (8)
-// decode warps of an SM share.  Chains of waits, not throughput, decided the design: a
+// behind, the issue slots of decode and promotion (a single CTA per tile was bound by the
+// latency of its activations, 36 KB a step: 1380 cycles a group); for few rows the decode,
+// which all decode warps of an SM share.  Chains of waits, not throughput, decided the design: a
 // step's decode takes ~1000 cycles from its words' arrival to the MMA, so NT teams keep NT
 // steps in flight, every stage has one barrier that says "filled" and one that says "free", and
 // the MMA issuer waits once per step.
@@ -52,6 +56,9 @@ constexpr int kDecSBO = kStepK / 8 * 128 + 16; // next 8 columns; the pad spread
 constexpr int kDecBytes = BN / 8 * kDecSBO;    // 16640
 constexpr int kWordBytes = kStepK / int4::kRowsPerWord * BN * 4;  // 4 KB
 constexpr int kMaxExperts = 1024;
+// an epilogue block: 8 rows x 128 fp32 columns, the right half 16 words further on (a warp's
+// 16 + 16 columns then lie in different banks)
+constexpr int kOutRow = BN + 16, kOutRows = 8, kOutBytes = kOutRows * kOutRow * 4;
 
 // Threads, rings and register shares by the rows of a tile.  kRegs*: setmaxnreg values (0: not
 // used), whose sum over the warps stays within what the block launches with.
@@ -59,7 +66,7 @@ template <int MT_>
 struct Cfg;
 template <>
 struct Cfg<256> {
-    static constexpr int MT = 256, NT = 2, NP = 8, kSteps = 4, kWords = 6, kAccBufs = 2, kCtasPerSm = 1;
+    static constexpr int MT = 256, NT = 2, NP = 8, kSteps = 5, kWords = 6, kAccBufs = 2, kCtasPerSm = 1;
     static constexpr int kRegsPromote = 168, kRegsOther = 48;
 };
 template <>
@@ -87,7 +94,9 @@ struct Plan : Cfg<MT> {
     static constexpr int kTmemCols = MT * C::kAccBufs;
     static constexpr int kBoxRows = MT < 64 ? MT : 64;
     static constexpr int kBoxBytes = kBoxRows * kStepK * 2;
-    static constexpr int kABytes = MT * kStepK * 2;
+    static constexpr bool kPair = MT == 256;      // two CTAs share the activations
+    static constexpr int kCtas = kPair ? 2 : 1;
+    static constexpr int kABytes = MT / kCtas * kStepK * 2;
     static constexpr int kLaunchRegs = 65536 / kThreads / C::kCtasPerSm / 8 * 8;
     static_assert(C::kRegsPromote * C::NP * 32 + C::kRegsOther * (kWarps - C::NP) * 32 <= kLaunchRegs * kThreads,
                   "register shares");
@@ -97,9 +106,11 @@ struct Plan : Cfg<MT> {
     static constexpr int words = dec + C::kSteps * kDecBytes;
     static constexpr int bars = words + C::kWords * kWordBytes;
     static constexpr int first = bars + 512;  // grouped: first tile of every expert
-    static constexpr int total = first + (kMaxExperts + 1) * 4 + 1024;  // + alignment slack
+    // the epilogue's blocks: two of 8 rows for every 4 promotion warps
+    static constexpr int out = (first + (kMaxExperts + 1) * 4 + 15) / 16 * 16;
+    static constexpr int total = out + C::NP / 4 * 2 * kOutBytes + 1024;  // + alignment slack
     static_assert(total <= 227 * 1024, "shared memory");
-    static_assert(MT * BN * 4 <= words, "the split's sums reuse the stages");
+    static_assert(kPair || MT * BN * 4 <= words, "the split's sums reuse the stages");
     static_assert(kTmemCols * C::kCtasPerSm <= 512 && (kTmemCols & (kTmemCols - 1)) == 0, "TMEM");
     static_assert((2 * C::kSteps + 2 * C::kWords + 2 * C::kAccBufs) * 8 + 4 <= 512, "barriers");
 };
@@ -200,16 +211,80 @@ __device__ __forceinline__ void store(const Params &p, size_t i, float v, float 
     else reinterpret_cast<uint16_t *>(p.C)[i] = DT::fromf(v);
 }
 
+// ---- what a pair's CTAs do through the first one ------------------------------------------
+__device__ __forceinline__ uint32_t in_first_cta(const void *p) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;\n" : "=r"(r) : "r"(tc::smem_addr(p)));
+    return r;
+}
+// Arrive on the barrier that the MMA issuer waits for.  Before it the arriving warp has made its
+// shared-memory stores visible to the async proxy (decode) or ordered its TMEM loads (promotion),
+// and the issuer touches that memory through MMAs only; a .release.cluster here would flush
+// all of the warp's memory operations first (~1300 cycles a step, a third of the GEMM's time).
+template <bool PAIR>
+__device__ __forceinline__ void arrive_at_issuer(uint64_t *bar) {
+    if constexpr (PAIR)
+        asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(in_first_cta(bar)) : "memory");
+    else tc::mbar_arrive(bar);
+}
+// TMA load into this CTA's shared memory, counted on the issuer's barrier
+template <bool PAIR>
+__device__ __forceinline__ void load_rows(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
+    if constexpr (PAIR)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+            "%3}], [%4];\n" ::"r"(tc::smem_addr(dst)),
+            "l"(map), "r"(x), "r"(y), "r"(in_first_cta(bar))
+            : "memory");
+    else tc::tma_load_2d(dst, map, x, y, bar);
+}
+template <bool PAIR>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+    else tc::mma_ss_f16(d, a, b, idesc, accumulate);
+}
+// arrive on *bar (of both CTAs of a pair) when the MMAs issued so far are through
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint64_t *bar) {
+    if constexpr (PAIR)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(
+                tc::smem_addr(bar)),
+            "h"((uint16_t)3)
+            : "memory");
+    else tc::mma_commit(bar);
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_alloc(uint32_t *slot, uint32_t ncols) {
+    if constexpr (PAIR) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc::smem_addr(slot)),
+                     "r"(ncols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::);
+    } else {
+        tc::tmem_alloc(slot, ncols);
+    }
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_dealloc(uint32_t base, uint32_t ncols) {
+    if constexpr (PAIR)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(base), "r"(ncols));
+    else tc::tmem_dealloc(base, ncols);
+}
+
 struct Tile {
     int n0, m0, rows, expert;
 };
 
 // tile t: row tile t / strips, column strip t % strips (neighbours share their rows)
 template <int MT>
-__device__ __forceinline__ Tile tile_of(const Params &p, const int *first, int t) {
+__device__ __forceinline__ Tile tile_of(const Params &p, const int *first, int t, int rank) {
     const int r = t / p.strips;
     Tile ti;
-    ti.n0 = (t - r * p.strips) * BN;
+    ti.n0 = ((t - r * p.strips) * Plan<MT>::kCtas + rank) * BN;
     ti.expert = 0;
     ti.m0 = r * MT;
     int end = p.M;
@@ -237,7 +312,9 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
     char *smem = smem_raw + ((1024u - (tc::smem_addr(smem_raw) & 1023u)) & 1023u);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int G = p.K / kGS;
-    const int sk = blockIdx.x % p.SK;
+    constexpr bool PAIR = C::kPair;
+    const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;  // in the pair; the first one issues the MMAs
+    const int sk = PAIR ? 0 : blockIdx.x % p.SK;
     const int g0 = (int)((long long)G * sk / p.SK), ng = (int)((long long)G * (sk + 1) / p.SK) - g0;
 
     uint64_t *ready = reinterpret_cast<uint64_t *>(smem + C::bars);  // a step's operands are in place
@@ -251,7 +328,8 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
 
     if (tid == 0) {
         for (int s = 0; s < C::kSteps; ++s) {
-            tc::mbar_init(&ready[s], 1 + 4);  // the activations' producer and the decode team's warps
+            // the (first) CTA's activations and the decode team's warps (of both CTAs)
+            tc::mbar_init(&ready[s], 1 + 4 * C::kCtas);
             tc::mbar_init(&done[s], 1);
         }
         for (int s = 0; s < C::kWords; ++s) {
@@ -260,11 +338,11 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
         }
         for (int b = 0; b < C::kAccBufs; ++b) {
             tc::mbar_init(&acc_full[b], 1);
-            tc::mbar_init(&acc_empty[b], C::NP);
+            tc::mbar_init(&acc_empty[b], C::NP * C::kCtas);
         }
         tc::fence_mbar_init();
     }
-    if (warp == 3) tc::tmem_alloc(tmem_slot, C::kTmemCols);
+    if (warp == 3) tmem_alloc<PAIR>(tmem_slot, C::kTmemCols);
     if (p.meta) {
         pdl_wait();  // meta comes from the routing kernel
         if (warp == 0) {
@@ -290,10 +368,12 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
     }
     tc::fence_before_sync();
     __syncthreads();
+    if (PAIR) gemv::cluster_sync_all();  // the other CTA's barriers are initialised
     tc::fence_after_sync();
     const uint32_t tmem = *tmem_slot;
     const int ntiles = (p.meta ? first[p.E] : (p.M + MT - 1) / MT) * p.strips;
-    const int t0 = blockIdx.x / p.SK, tstep = gridDim.x / p.SK;
+    const int per_tile = PAIR ? 2 : p.SK;
+    const int t0 = blockIdx.x / per_tile, tstep = gridDim.x / per_tile;
 
     // promotion threads: row r of the M operand (a column of C) and the tile's activation rows
     // jbase .. jbase + kCols - 1
@@ -310,38 +390,41 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
             Ring<C::kSteps> q;
             bool ok = true;
             for (int t = t0; t < ntiles && ok; t += tstep) {
-                const Tile ti = tile_of<MT>(p, first, t);
-                const int boxes = (ti.rows + C::kBoxRows - 1) / C::kBoxRows;
+                const Tile ti = tile_of<MT>(p, first, t, rank);
+                // a pair's CTA holds half of the MMA's N rows
+                const int nrows = PAIR ? (ti.rows + 31) / 32 * 16 : ti.rows;
+                const int boxes = (nrows + C::kBoxRows - 1) / C::kBoxRows;
                 for (int x = 0; x < 2 * ng; ++x, q.advance()) {
                     if (!tc::mbar_wait(&done[q.i], q.parity ^ 1u)) {
                         ok = false;
                         break;
                     }
                     if (elect_one()) {
-                        tc::mbar_expect_tx(&ready[q.i], boxes * C::kBoxBytes);
+                        if (rank == 0) tc::mbar_expect_tx(&ready[q.i], C::kCtas * boxes * C::kBoxBytes);
                         char *a = smem + C::a + q.i * C::kABytes;
                         for (int b = 0; b < boxes; ++b)
-                            tc::tma_load_2d(a + b * C::kBoxBytes, &tmA, g0 * kGS + x * kStepK,
-                                            ti.m0 + b * C::kBoxRows, &ready[q.i]);
+                            load_rows<PAIR>(a + b * C::kBoxBytes, &tmA, g0 * kGS + x * kStepK,
+                                            ti.m0 + rank * nrows + b * C::kBoxRows, &ready[q.i]);
                     }
                     __syncwarp();
                 }
             }
-            if (!ok) {  // copies still in flight must land before the block can exit
+            if (!ok && rank == 0) {  // copies still in flight must land before the blocks can exit
                 for (int s = 0; s < C::kSteps; ++s) {
                     q.advance();
                     tc::mbar_wait(&ready[q.i], q.parity ^ 1u);
                 }
             }
-        } else if (warp == 1) {
+        } else if (warp == 1 && rank == 0) {
             // ---------------- MMA issuer ----------------
             Ring<C::kSteps> q;
             Ring<C::kAccBufs> b;
             bool ok = true;
             for (int t = t0; t < ntiles && ok; t += tstep) {
-                const Tile ti = tile_of<MT>(p, first, t);
+                const Tile ti = tile_of<MT>(p, first, t, rank);
                 // M operand MN-major (bit 15), N operand K-major
-                const uint32_t idesc = tc::idesc_f16(DT::kBF16, BN, (ti.rows + 15) & ~15) | (1u << 15);
+                const int nrows = PAIR ? (ti.rows + 31) & ~31 : (ti.rows + 15) & ~15;
+                const uint32_t idesc = tc::idesc_f16(DT::kBF16, BN * C::kCtas, nrows) | (1u << 15);
                 for (int x = 0; x < 2 * ng; ++x, q.advance()) {
                     if (!(x & 1) && !tc::mbar_wait(&acc_empty[b.i], b.parity ^ 1u)) {
                         ok = false;
@@ -359,10 +442,10 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
                         // (addresses stay below 2^18: a step along K adds to the address field only)
 #pragma unroll
                         for (int kk = 0; kk < kStepK / 16; ++kk)
-                            tc::mma_ss_f16(tmem + b.i * MT, w + (uint64_t)(kk * 2 * kDecLBO / 16),
-                                           v + (uint64_t)(kk * 2), idesc, ((x & 1) | kk) != 0);
-                        tc::mma_commit(&done[q.i]);
-                        if (x & 1) tc::mma_commit(&acc_full[b.i]);
+                            mma<PAIR>(tmem + b.i * MT, w + (uint64_t)(kk * 2 * kDecLBO / 16), v + (uint64_t)(kk * 2),
+                                      idesc, ((x & 1) | kk) != 0);
+                        commit<PAIR>(&done[q.i]);
+                        if (x & 1) commit<PAIR>(&acc_full[b.i]);
                     }
                     __syncwarp();
                     if (x & 1) b.advance();
@@ -373,7 +456,7 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
             Ring<C::kWords> q;
             bool ok = true;
             for (int t = t0; t < ntiles && ok; t += tstep) {
-                const Tile ti = tile_of<MT>(p, first, t);
+                const Tile ti = tile_of<MT>(p, first, t, rank);
                 const int row0 = (ti.expert * G + g0) * int4::kWordsPerGroup;
                 for (int x = 0; x < 2 * ng; ++x, q.advance()) {
                     if (!tc::mbar_wait(&words_empty[q.i], q.parity ^ 1u)) {
@@ -433,7 +516,7 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
                 tc::fence_proxy_async_smem();
                 __syncwarp();
                 if (elect_one()) {
-                    tc::mbar_arrive(&ready[q.i]);
+                    arrive_at_issuer<PAIR>(&ready[q.i]);
                     tc::mbar_arrive(&words_empty[qw.i]);
                 }
                 __syncwarp();
@@ -450,7 +533,7 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
         uint16_t sc[kAhead];
         const uint16_t *sp = nullptr;
         auto scales_of = [&](int t) {
-            const Tile ti = tile_of<MT>(p, first, t);
+            const Tile ti = tile_of<MT>(p, first, t, rank);
             const int n = ti.n0 + col;
             sp = p.S + ((size_t)ti.expert * G + g0) * p.N + (n < p.N ? n : 0);
 #pragma unroll
@@ -458,10 +541,9 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
         };
         if (t0 < ntiles) scales_of(t0);
         Ring<C::kAccBufs> b;
-        bool ok = true;
-        for (int t = t0; t < ntiles && ok; t += tstep) {
-            const Tile ti = tile_of<MT>(p, first, t);
-            const int n = ti.n0 + col;
+        bool ok = true;  // (a warp whose wait timed out still meets the others at their barriers)
+        for (int t = t0; t < ntiles; t += tstep) {
+            const Tile ti = tile_of<MT>(p, first, t, rank);
             uint64_t acc[C::kCols / 2];
 #pragma unroll
             for (int j = 0; j < C::kCols / 2; ++j) acc[j] = 0ull;
@@ -494,12 +576,12 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
                     }
                     tc::fence_before_sync();
                     __syncwarp();
-                    if (elect_one()) tc::mbar_arrive(&acc_empty[b.i]);
+                    if (elect_one()) arrive_at_issuer<PAIR>(&acc_empty[b.i]);
                     __syncwarp();
                     b.advance();
                 }
             }
-            if (p.SK > 1) {
+            if (!PAIR && p.SK > 1) {
                 // one tile: its sums [rows][128] go into the stages, whose last readers (the MMAs of the
                 // last group) are through, and are joined below
                 float *part = reinterpret_cast<float *>(smem);
@@ -514,33 +596,85 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
             }
             if (t + tstep < ntiles) scales_of(t + tstep);
             pdl_wait();
-            if (n < p.N) {
-                constexpr int kBatch = MT == 32 ? 8 : 16;  // rows whose epilogue operands are in flight together
-                const size_t i0 = (size_t)(ti.m0 + jbase) * p.N + n;
+            // 16 rows at a time through shared memory, so that a thread takes 8 columns of two rows
+            // (storing TMEM lanes directly, 2 bytes a lane, took 20,000-31,000 cycles a tile)
+            char *blocks = smem + C::out + (pw >> 2) * 2 * kOutBytes;
+            const int th = (pw & 3) * 32 + lane, row = th >> 4, cb = th & 15;
+            const int on = ti.n0 + 8 * cb, sw = (cb >> 2) & 1;
+            constexpr bool kOther = POSTOP == 1 || POSTOP == 2;
+            uint4 other[2];
+            auto fetch = [&](int c) {
 #pragma unroll
-                for (int c = 0; c < C::kCols; c += kBatch) {
-                    float e[kBatch];
+                for (int h = 0; h < 2; ++h) {
+                    const int m = jbase + (c + h) * kOutRows + row;
+                    if (kOther && m < ti.rows && on < p.N)
+                        other[h] = __ldg(reinterpret_cast<const uint4 *>(p.Other + (size_t)(ti.m0 + m) * p.N + on));
+                }
+            };
+            fetch(0);
 #pragma unroll
-                    for (int j = 0; j < kBatch; ++j)
-                        e[j] = (POSTOP == 1 || POSTOP == 2) && jbase + c + j >= ti.rows
-                                   ? 0.0f
-                                   : epi_in<DT, POSTOP, OUT_F32>(p.Other, p.Bias, i0 + (size_t)(c + j) * p.N, n);
+            for (int c = 0; c < C::kCols / kOutRows; c += 2) {
+                if (jbase + c * kOutRows >= ti.rows) continue;  // the same for the four warps that share the blocks
+                if (c) asm volatile("bar.sync %0, 128;\n" ::"r"(1 + (pw >> 2)) : "memory");  // read by all
 #pragma unroll
-                    for (int j = 0; j < kBatch; j += 2) {
-                        float v0, v1;
-                        unpack2(acc[(c + j) / 2], v0, v1);
-                        const size_t i = i0 + (size_t)(c + j) * p.N;
-                        if (jbase + c + j < ti.rows) store<DT, POSTOP, OUT_F32>(p, i, v0, e[j]);
-                        if (jbase + c + j + 1 < ti.rows) store<DT, POSTOP, OUT_F32>(p, i + p.N, v1, e[j + 1]);
+                for (int j = 0; j < 2 * kOutRows; j += 2) {
+                    float *mine = reinterpret_cast<float *>(blocks + (j / kOutRows) * kOutBytes) + col +
+                                  ((col >> 6) << 4) + (j % kOutRows) * kOutRow;
+                    float v0, v1;
+                    unpack2(acc[(c * kOutRows + j) / 2], v0, v1);
+                    mine[0] = v0;
+                    mine[kOutRow] = v1;
+                }
+                asm volatile("bar.sync %0, 128;\n" ::"r"(1 + (pw >> 2)) : "memory");
+                float v[2][8];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float4 *src = reinterpret_cast<const float4 *>(blocks + h * kOutBytes) +
+                                        (row * kOutRow + 8 * cb + ((cb >> 3) << 4)) / 4;
+                    const float4 x0 = src[sw], x1 = src[sw ^ 1];
+                    const float4 lo = sw ? x1 : x0, hi = sw ? x0 : x1;
+                    v[h][0] = lo.x, v[h][1] = lo.y, v[h][2] = lo.z, v[h][3] = lo.w;
+                    v[h][4] = hi.x, v[h][5] = hi.y, v[h][6] = hi.z, v[h][7] = hi.w;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        float e;
+                        if constexpr (kOther) {
+                            const uint32_t ow[4] = {other[h].x, other[h].y, other[h].z, other[h].w};
+                            e = DT::tof((uint16_t)((k & 1) ? ow[k / 2] >> 16 : ow[k / 2] & 0xFFFFu));
+                        } else {
+                            e = on < p.N ? epi_in<DT, POSTOP, OUT_F32>(p.Other, p.Bias, 0, on + k) : 0.0f;
+                        }
+                        v[h][k] = epi<POSTOP, OUT_F32>(v[h][k], e);
+                    }
+                }
+                fetch(c + 2);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int m = jbase + (c + h) * kOutRows + row;
+                    if (!ok || m >= ti.rows || on >= p.N) continue;
+                    const size_t i = (size_t)(ti.m0 + m) * p.N + on;
+                    if constexpr (OUT_F32) {
+                        float4 *dst = reinterpret_cast<float4 *>(reinterpret_cast<float *>(p.C) + i);
+                        dst[0] = make_float4(v[h][0], v[h][1], v[h][2], v[h][3]);
+                        dst[1] = make_float4(v[h][4], v[h][5], v[h][6], v[h][7]);
+                    } else {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            w[k] = (uint32_t)DT::fromf(v[h][2 * k]) | ((uint32_t)DT::fromf(v[h][2 * k + 1]) << 16);
+                        *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(p.C) + i) =
+                            make_uint4(w[0], w[1], w[2], w[3]);
                     }
                 }
             }
+            // the next tile writes the blocks again
+            asm volatile("bar.sync %0, 128;\n" ::"r"(1 + (pw >> 2)) : "memory");
         }
         pdl_launch_dependents();
         regs_dec<C::kRegsOther>();  // every warp goes on with the same share
     }
-    if (p.SK > 1) {
-        const Tile ti = tile_of<MT>(p, first, t0);
+    if (!PAIR && p.SK > 1) {
+        const Tile ti = tile_of<MT>(p, first, t0, rank);
         const float *part = reinterpret_cast<const float *>(smem);
         __syncthreads();
         gemv::cluster_sync_all();
@@ -558,9 +692,10 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
     }
     tc::fence_before_sync();
     __syncthreads();
+    if (PAIR) gemv::cluster_sync_all();  // neither CTA leaves while the other may use its memory
     if (warp == 3) {
         tc::fence_after_sync();
-        tc::tmem_dealloc(tmem, C::kTmemCols);
+        tmem_dealloc<PAIR>(tmem, C::kTmemCols);
     }
 }
 
@@ -575,12 +710,13 @@ cudaError_t launch(const GemvArgs &a, int sms, const int *meta, int E) {
     e = tc::make_map_plain(&mapB, a.B, CU_TENSOR_MAP_DATA_TYPE_INT32, 4, (meta ? E : 1) * (a.K / int4::kRowsPerWord),
                            a.N, kStepK / int4::kRowsPerWord, BN);
     if (e != cudaSuccess) return e;
-    const int strips = (a.N + BN - 1) / BN;
+    const int strips = (a.N + BN * C::kCtas - 1) / (BN * C::kCtas);
     const Params p{(const uint16_t *)a.S, a.C, (const uint16_t *)a.Other, a.Bias, a.M, a.N, a.K, a.SK, strips, meta, E};
     // grouped: an upper bound, every expert adds at most one partial tile
     const long long tiles = ((long long)(a.M + MT - 1) / MT + (meta ? E : 0)) * strips;
-    const long long slots = (long long)sms * C::kCtasPerSm;
-    const int grid = a.SK > 1 ? (int)tiles * a.SK : (int)(tiles < slots ? tiles : slots);
+    const long long slots = (long long)sms * C::kCtasPerSm / C::kCtas;
+    const int per_tile = C::kPair ? 2 : a.SK;  // CTAs of a cluster
+    const int grid = (int)(a.SK > 1 || tiles < slots ? tiles : slots) * per_tile;
     return dispatch_epilogue<GemvArgs>(a, [&](auto dt, auto po, auto of) -> cudaError_t {
         using DT = typename decltype(dt)::type;
         auto kern = gemm_int4_kernel<MT, DT, decltype(po)::value, decltype(of)::value>;
@@ -593,8 +729,8 @@ cudaError_t launch(const GemvArgs &a, int sms, const int *meta, int E) {
         }
         cudaError_t err = ensure_smem(kern, C::total);
         if (err != cudaSuccess) return err;
-        return launch_kernel_cluster(kern, dim3(grid), dim3(C::kThreads), (size_t)C::total, a.stream, dim3(a.SK, 1, 1),
-                                     p, mapA, mapB);
+        return launch_kernel_cluster(kern, dim3(grid), dim3(C::kThreads), (size_t)C::total, a.stream,
+                                     dim3(per_tile, 1, 1),                                     p, mapA, mapB);
     });
 }
 
@@ -604,11 +740,18 @@ cudaError_t int4_gemm_launch(const GemvArgs &a, int sms, const int *meta, int E)
     GemvArgs b = a;
     // activation rows per tile: what the rows (grouped: an expert's average) fill
     const long long per = meta ? (a.M + E - 1) / E : a.M;
-    const int MT = per <= 32 ? 32 : per <= 64 ? 64 : per <= 128 ? 128 : 256;
+    int MT = per <= 32 ? 32 : per <= 64 ? 64 : per <= 128 ? 128 : 256;
+    const long long strips = (a.N + gemm4::BN - 1) / gemm4::BN;
+    if (MT == 256 && !meta) {
+        // a pair of CTAs takes a group of 256 x 256 in ~1.5 times a CTA's 128 x 128
+        const long long pairs = (strips + 1) / 2 * ((a.M + 255) / 256), singles = strips * ((a.M + 127) / 128);
+        const long long pair_waves = (2 * pairs + sms - 1) / sms, waves = (singles + sms - 1) / sms;
+        if (3 * pair_waves > 2 * waves) MT = 128;
+    }
     // K split over a cluster while the tiles leave SMs without work
-    const long long tiles = (long long)((a.N + gemm4::BN - 1) / gemm4::BN) * ((a.M + MT - 1) / MT);
+    const long long tiles = strips * ((a.M + MT - 1) / MT);
     int sk = 1;
-    if (!meta)
+    if (!meta && MT < 256)
         while (sk < 8 && 2 * sk <= a.K / kGS && tiles * 2 * sk <= sms) sk *= 2;
     b.SK = sk;
     return MT == 32    ? gemm4::launch<32>(b, sms, meta, E)
