@@ -136,3 +136,23 @@ def test_long_batches_streams_and_graphs(cuda, tl):
     graph.replay()
     assert torch.equal(ids, i3) and torch.equal(w, w3)
     assert tl.moe_topk(logits[:0], 8, **how)[0].shape == (0, 8)
+
+
+@pytest.mark.parametrize("E,topk,scoring,biased,groups", [
+    (128, 8, "softmax", False, {}), (128, 15, "sigmoid", True, {}), (16, 4, "softmax", True, {}),
+    (500, 6, "softmax", False, {}), (9, 9, "sigmoid", True, {}), (257, 16, "softmax", True, {}),
+    (256, 8, "softmax", True, dict(n_group=8, topk_group=4, group_top=2)),
+    (96, 6, "sigmoid", False, dict(n_group=12, topk_group=3, group_top=1)),
+    (384, 8, "sigmoid", True, dict(n_group=3, topk_group=2, group_top=2))])
+def test_many_tokens(cuda, tl, E, topk, scoring, biased, groups):
+    """Batches long enough for the form with two tokens per warp (an odd number of them)."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(E)
+    for dtype in TYPES:
+        logits = (2.0 * torch.randn(2051, E, generator=g, device="cuda")).to(dtype)
+        logits[5] = float("-inf")
+        logits[6, : E // 2] = float("nan")
+        logits[7, 3] = float("inf")
+        logits[-1] = 0.5
+        bias = 0.1 * torch.randn(E, generator=g, device="cuda") if biased else None
+        run(tl, logits, topk, bias=bias, scoring=scoring, renormalize=dtype != torch.float16, **groups)
