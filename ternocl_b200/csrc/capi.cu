@@ -5,6 +5,7 @@
 // codes from a stream-ordered pool (scratch_alloc below).
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
@@ -207,9 +208,10 @@ static GemvPlan gemv_i4_plan(int M, int N, int K) {
     const int G = K / kGS, sms = sm_count();
     const long long tiles = (long long)((N + 31) / 32) * ((M + 7) / 8);
     GemvPlan p;
-    p.warps = tiles >= 4LL * sms ? 4 : 8;
-    p.SK = tiles < sms && G >= 2 ? 2 : 1;
-    while (p.SK < G && p.SK < kMaxClusterSK && int4_gemv_smem(M, K, p.SK, p.warps) > kGemvSmemBudget) ++p.SK;
+    p.warps = options().gemv_warps ? (options().gemv_warps >= 8 ? 8 : 4) : 8;
+    p.SK = 1;
+    while (p.SK < kMaxClusterSK && 2 * p.SK * p.warps <= G && tiles * p.SK * 2 <= 3LL * sms) p.SK *= 2;
+    if (options().gemv_split) p.SK = std::min({(int)options().gemv_split, G, kMaxClusterSK});
     p.cluster = p.SK > 1;
     return p;
 }
@@ -775,11 +777,6 @@ int ternocl_int4_upcvt(const void *A, const uint32_t *B, const void *S, void *C,
     if (algo == TERNOCL_ALGO_GEMM || (algo == TERNOCL_ALGO_AUTO && M > kInt4GemvMaxM))
         return cuda_status(int4_gemm_launch(a, sm_count()));
     const GemvPlan p = gemv_i4_plan(M, N, K);
-    if (int4_gemv_smem(M, K, p.SK, p.warps) > 227 * 1024) {
-        // (a K of more than 70,000 at M = 8: the GEMM walks any K)
-        if (algo == TERNOCL_ALGO_GEMV) return TERNOCL_ERR_WORKSPACE;
-        return cuda_status(int4_gemm_launch(a, sm_count()));
-    }
     a.SK = p.SK;
     a.warps = p.warps;
     a.cluster = p.cluster ? 1 : 0;
@@ -817,7 +814,7 @@ int ternocl_moe_decode_gate_up_int4(const int32_t *ids, const void *X, const uin
         !aligned(H, 2) || !aligned(ids, 4))
         return TERNOCL_ERR_ARG;
     return cuda_status(moe_decode_gate_up_int4_launch(ids, X, Bg, Sg, Bu, Su, H, G, N, K, topk, num_experts, dtype,
-                                                      (cudaStream_t)stream));
+                                                      sm_count(), (cudaStream_t)stream));
 }
 
 int ternocl_moe_decode_down_sum_int4(const int32_t *ids, const void *H, const void *RW, const uint32_t *B,
@@ -834,7 +831,7 @@ int ternocl_moe_decode_down_sum_int4(const int32_t *ids, const void *H, const vo
         !aligned(ids, 4))
         return TERNOCL_ERR_ARG;
     return cuda_status(moe_decode_down_sum_int4_launch(ids, H, RW, B, S, O, T, N, K, topk, num_experts, dtype,
-                                                       (cudaStream_t)stream));
+                                                       sm_count(), (cudaStream_t)stream));
 }
 
 // ---- the experts' choice ----

@@ -72,12 +72,12 @@ __device__ __forceinline__ float epi_in(const uint16_t *__restrict__ other,
 }
 
 // Apply the epilogue to element (m, n) of C and store it (DT or fp32).
-template <class DT, int POSTOP, bool OUT_F32>
+template <class DT, int POSTOP, bool OUT_F32, bool ACCURATE = false>
 __device__ __forceinline__ void epi_store(void *__restrict__ C, const uint16_t *__restrict__ other,
                                           const void *__restrict__ bias, int N, int m, int n,
                                           float v) {
     const size_t i = (size_t)m * N + n;
-    v = epi<POSTOP>(v, epi_in<DT, POSTOP, OUT_F32>(other, bias, i, n));
+    v = epi<POSTOP, ACCURATE>(v, epi_in<DT, POSTOP, OUT_F32>(other, bias, i, n));
     if constexpr (OUT_F32) reinterpret_cast<float *>(C)[i] = v;
     else reinterpret_cast<uint16_t *>(C)[i] = DT::fromf(v);
 }

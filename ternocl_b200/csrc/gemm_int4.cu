@@ -25,8 +25,9 @@
 //               matrix of the M operand (MN-major) out of 8 words;
 //   NP warps    promotion: tcgen05.ld of a finished group, acc += S * D_g (f32x2), and at the
 //               tile's end the epilogue, while the other roles run on into the next tile.
-// Few tiles split K over a thread-block cluster: its CTAs leave their sums in shared memory
-// and each adds up a share of the rows in split order over distributed shared memory.
+// The tiles of the last round, when they would leave CTAs without work, are split along K over
+// the CTAs of a cluster: these leave their sums in shared memory and each adds up a share of
+// the rows in split order over distributed shared memory.
 //
 // What bounds it: for many rows the MMAs (1024 cycles for a group at MT = 256) and, close
 // behind, the issue slots of decode and promotion (a single CTA per tile was bound by the
@@ -39,6 +40,9 @@
 // wait (bounded) for their copies in flight, and TMEM is freed.
 #include <cuda.h>
 #include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "gemv_common.cuh"
@@ -60,28 +64,30 @@ constexpr int kMaxExperts = 1024;
 // 16 + 16 columns then lie in different banks)
 constexpr int kOutRow = BN + 16, kOutRows = 8, kOutBytes = kOutRows * kOutRow * 4;
 
-// Threads, rings and register shares by the rows of a tile.  kRegs*: setmaxnreg values (0: not
-// used), whose sum over the warps stays within what the block launches with.
+// Threads, rings and register shares by the rows of a tile; one CTA per SM.  kRegs*: setmaxnreg
+// values (0: not used), whose sum over the warps stays within what the block launches with.
+// Few rows leave shared memory for words: 64 to 80 KB of them on their way cover the ~1.2 us
+// that they take from HBM.
 template <int MT_>
 struct Cfg;
 template <>
 struct Cfg<256> {
-    static constexpr int MT = 256, NT = 2, NP = 8, kSteps = 5, kWords = 6, kAccBufs = 2, kCtasPerSm = 1;
+    static constexpr int MT = 256, NT = 2, NP = 8, kSteps = 5, kWords = 6, kAccBufs = 2;
     static constexpr int kRegsPromote = 168, kRegsOther = 48;
 };
 template <>
 struct Cfg<128> {
-    static constexpr int MT = 128, NT = 3, NP = 8, kSteps = 5, kWords = 6, kAccBufs = 4, kCtasPerSm = 1;
+    static constexpr int MT = 128, NT = 3, NP = 8, kSteps = 4, kWords = 16, kAccBufs = 4;
     static constexpr int kRegsPromote = 112, kRegsOther = 64;
 };
 template <>
 struct Cfg<64> {
-    static constexpr int MT = 64, NT = 4, NP = 4, kSteps = 6, kWords = 8, kAccBufs = 4, kCtasPerSm = 1;
+    static constexpr int MT = 64, NT = 4, NP = 4, kSteps = 5, kWords = 20, kAccBufs = 4;
     static constexpr int kRegsPromote = 112, kRegsOther = 72;
 };
 template <>
 struct Cfg<32> {
-    static constexpr int MT = 32, NT = 2, NP = 4, kSteps = 4, kWords = 4, kAccBufs = 4, kCtasPerSm = 2;
+    static constexpr int MT = 32, NT = 4, NP = 4, kSteps = 6, kWords = 20, kAccBufs = 4;
     static constexpr int kRegsPromote = 0, kRegsOther = 0;
 };
 
@@ -97,7 +103,7 @@ struct Plan : Cfg<MT> {
     static constexpr bool kPair = MT == 256;      // two CTAs share the activations
     static constexpr int kCtas = kPair ? 2 : 1;
     static constexpr int kABytes = MT / kCtas * kStepK * 2;
-    static constexpr int kLaunchRegs = 65536 / kThreads / C::kCtasPerSm / 8 * 8;
+    static constexpr int kLaunchRegs = 65536 / kThreads / 8 * 8;
     static_assert(C::kRegsPromote * C::NP * 32 + C::kRegsOther * (kWarps - C::NP) * 32 <= kLaunchRegs * kThreads,
                   "register shares");
     // shared memory: 1024-byte aligned A stages first
@@ -111,7 +117,8 @@ struct Plan : Cfg<MT> {
     static constexpr int total = out + C::NP / 4 * 2 * kOutBytes + 1024;  // + alignment slack
     static_assert(total <= 227 * 1024, "shared memory");
     static_assert(kPair || MT * BN * 4 <= words, "the split's sums reuse the stages");
-    static_assert(kTmemCols * C::kCtasPerSm <= 512 && (kTmemCols & (kTmemCols - 1)) == 0, "TMEM");
+    static_assert(C::NT <= C::kSteps && C::NT <= C::kWords, "decode teams");
+    static_assert(kTmemCols <= 512 && (kTmemCols & (kTmemCols - 1)) == 0, "TMEM");
     static_assert((2 * C::kSteps + 2 * C::kWords + 2 * C::kAccBufs) * 8 + 4 <= 512, "barriers");
 };
 
@@ -120,7 +127,8 @@ struct Params {
     void *C;
     const uint16_t *Other;
     const void *Bias;
-    int M, N, K, SK, strips;
+    int M, N, K, strips;
+    int cluster;  // CTAs that may share a tile of the last round (a pair: 2, which share every tile)
     const int *meta;  // grouped: E+1 row offsets (moe_route's meta), else null
     int E;
 };
@@ -193,14 +201,6 @@ __device__ __forceinline__ void decode_half(const uint4 w0, const uint4 w1, int 
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) out[r] = make_uint4(d[0][r], d[1][r], d[2][r], d[3][r]);
-}
-
-__device__ __forceinline__ float ld_dsmem_f32(uint32_t local_addr, uint32_t rank) {
-    uint32_t remote;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(remote) : "r"(local_addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(remote));
-    return v;
 }
 
 // element i = m * N + n, e = its epilogue operand
@@ -277,13 +277,39 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t base, uint32_t ncols) {
 
 struct Tile {
     int n0, m0, rows, expert;
+    int g0, ng;  // the groups of this CTA
 };
 
-// tile t: row tile t / strips, column strip t % strips (neighbours share their rows)
+// The CTA's tiles: `full` rounds of one tile per CTA (or pair), then the rest, `split` CTAs of a
+// cluster per tile.
+struct Schedule {
+    int index, stride;       // of the CTA (or pair) among all
+    int full, split, items;  // items: the CTA's tiles
+    int rest;                // first tile of the last round
+    __device__ __forceinline__ Schedule(int ntiles, int unit, int units, int cluster, int groups) {
+        index = unit;
+        stride = units;
+        full = ntiles / units;
+        rest = full * units;
+        const int left = ntiles - rest;
+        split = 1;
+        while (2 * split <= cluster && 2 * split * left <= units && 2 * split <= groups) split *= 2;
+        if (left == 0) split = 1;
+        items = full + (unit / split < left ? 1 : 0);
+    }
+};
+
+// tile of item k: row tile t / strips, column strip t % strips (neighbours share their rows)
 template <int MT>
-__device__ __forceinline__ Tile tile_of(const Params &p, const int *first, int t, int rank) {
+__device__ __forceinline__ Tile tile_of(const Params &p, const int *first, const Schedule &s, int k, int rank) {
+    const int G = p.K / kGS;
+    const bool last = k == s.full;
+    const int t = last ? s.rest + s.index / s.split : k * s.stride + s.index;
+    const int sk = last ? s.index % s.split : 0, n = last ? s.split : 1;
     const int r = t / p.strips;
     Tile ti;
+    ti.g0 = (int)((long long)G * sk / n);
+    ti.ng = (int)((long long)G * (sk + 1) / n) - ti.g0;
     ti.n0 = ((t - r * p.strips) * Plan<MT>::kCtas + rank) * BN;
     ti.expert = 0;
     ti.m0 = r * MT;
@@ -305,7 +331,7 @@ __device__ __forceinline__ Tile tile_of(const Params &p, const int *first, int t
 }
 
 template <int MT, class DT, int POSTOP, bool OUT_F32>
-__global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
+__global__ void __launch_bounds__(Plan<MT>::kThreads, 1)
     gemm_int4_kernel(const Params p, const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB) {
     using C = Plan<MT>;
     extern __shared__ __align__(1024) char smem_raw[];
@@ -314,8 +340,6 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
     const int G = p.K / kGS;
     constexpr bool PAIR = C::kPair;
     const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;  // in the pair; the first one issues the MMAs
-    const int sk = PAIR ? 0 : blockIdx.x % p.SK;
-    const int g0 = (int)((long long)G * sk / p.SK), ng = (int)((long long)G * (sk + 1) / p.SK) - g0;
 
     uint64_t *ready = reinterpret_cast<uint64_t *>(smem + C::bars);  // a step's operands are in place
     uint64_t *done = ready + C::kSteps;                              // its MMAs have read them
@@ -372,8 +396,7 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
     tc::fence_after_sync();
     const uint32_t tmem = *tmem_slot;
     const int ntiles = (p.meta ? first[p.E] : (p.M + MT - 1) / MT) * p.strips;
-    const int per_tile = PAIR ? 2 : p.SK;
-    const int t0 = blockIdx.x / per_tile, tstep = gridDim.x / per_tile;
+    const Schedule sched(ntiles, blockIdx.x / C::kCtas, gridDim.x / C::kCtas, PAIR ? 1 : p.cluster, G);
 
     // promotion threads: row r of the M operand (a column of C) and the tile's activation rows
     // jbase .. jbase + kCols - 1
@@ -389,12 +412,12 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
             pdl_wait();
             Ring<C::kSteps> q;
             bool ok = true;
-            for (int t = t0; t < ntiles && ok; t += tstep) {
-                const Tile ti = tile_of<MT>(p, first, t, rank);
+            for (int k = 0; k < sched.items && ok; ++k) {
+                const Tile ti = tile_of<MT>(p, first, sched, k, rank);
                 // a pair's CTA holds half of the MMA's N rows
                 const int nrows = PAIR ? (ti.rows + 31) / 32 * 16 : ti.rows;
                 const int boxes = (nrows + C::kBoxRows - 1) / C::kBoxRows;
-                for (int x = 0; x < 2 * ng; ++x, q.advance()) {
+                for (int x = 0; x < 2 * ti.ng; ++x, q.advance()) {
                     if (!tc::mbar_wait(&done[q.i], q.parity ^ 1u)) {
                         ok = false;
                         break;
@@ -403,7 +426,7 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
                         if (rank == 0) tc::mbar_expect_tx(&ready[q.i], C::kCtas * boxes * C::kBoxBytes);
                         char *a = smem + C::a + q.i * C::kABytes;
                         for (int b = 0; b < boxes; ++b)
-                            load_rows<PAIR>(a + b * C::kBoxBytes, &tmA, g0 * kGS + x * kStepK,
+                            load_rows<PAIR>(a + b * C::kBoxBytes, &tmA, ti.g0 * kGS + x * kStepK,
                                             ti.m0 + rank * nrows + b * C::kBoxRows, &ready[q.i]);
                     }
                     __syncwarp();
@@ -417,48 +440,53 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
             }
         } else if (warp == 1 && rank == 0) {
             // ---------------- MMA issuer ----------------
+            // (one: a decode team waits for the parity of the last pass over its slot, which tells that
+            // pass from the one before only while the steps are done in order and NT <= kSteps)
             Ring<C::kSteps> q;
             Ring<C::kAccBufs> b;
             bool ok = true;
-            for (int t = t0; t < ntiles && ok; t += tstep) {
-                const Tile ti = tile_of<MT>(p, first, t, rank);
+            for (int k = 0; k < sched.items && ok; ++k) {
+                const Tile ti = tile_of<MT>(p, first, sched, k, rank);
                 // M operand MN-major (bit 15), N operand K-major
                 const int nrows = PAIR ? (ti.rows + 31) & ~31 : (ti.rows + 15) & ~15;
                 const uint32_t idesc = tc::idesc_f16(DT::kBF16, BN * C::kCtas, nrows) | (1u << 15);
-                for (int x = 0; x < 2 * ng; ++x, q.advance()) {
-                    if (!(x & 1) && !tc::mbar_wait(&acc_empty[b.i], b.parity ^ 1u)) {
+                for (int i = 0; i < ti.ng && ok; ++i, b.advance()) {
+                    if (!tc::mbar_wait(&acc_empty[b.i], b.parity ^ 1u)) {
                         ok = false;
                         break;
                     }
-                    if (!tc::mbar_wait(&ready[q.i], q.parity)) {
-                        ok = false;
-                        break;
-                    }
-                    tc::fence_after_sync();
-                    const uint64_t w = tc::sdesc_kmajor_noswz(tc::smem_addr(smem + C::dec + q.i * kDecBytes), kDecLBO,
-                                                              kDecSBO);
-                    const uint64_t v = tc::sdesc_kmajor_sw128(tc::smem_addr(smem + C::a + q.i * C::kABytes));
-                    if (elect_one()) {
-                        // (addresses stay below 2^18: a step along K adds to the address field only)
 #pragma unroll
-                        for (int kk = 0; kk < kStepK / 16; ++kk)
-                            mma<PAIR>(tmem + b.i * MT, w + (uint64_t)(kk * 2 * kDecLBO / 16), v + (uint64_t)(kk * 2),
-                                      idesc, ((x & 1) | kk) != 0);
-                        commit<PAIR>(&done[q.i]);
-                        if (x & 1) commit<PAIR>(&acc_full[b.i]);
+                    for (int h = 0; h < 2; ++h) {
+                        if (!tc::mbar_wait(&ready[q.i], q.parity)) {
+                            ok = false;
+                            break;
+                        }
+                        tc::fence_after_sync();
+                        const uint64_t w = tc::sdesc_kmajor_noswz(tc::smem_addr(smem + C::dec + q.i * kDecBytes),
+                                                                  kDecLBO, kDecSBO);
+                        const uint64_t v = tc::sdesc_kmajor_sw128(tc::smem_addr(smem + C::a + q.i * C::kABytes));
+                        if (elect_one()) {
+                            // (addresses stay below 2^18: a step along K adds to the address field only)
+#pragma unroll
+                            for (int kk = 0; kk < kStepK / 16; ++kk)
+                                mma<PAIR>(tmem + b.i * MT, w + (uint64_t)(kk * 2 * kDecLBO / 16), v + (uint64_t)(kk * 2),
+                                          idesc, (h | kk) != 0);
+                            commit<PAIR>(&done[q.i]);
+                            if (h) commit<PAIR>(&acc_full[b.i]);
+                        }
+                        __syncwarp();
+                        q.advance();
                     }
-                    __syncwarp();
-                    if (x & 1) b.advance();
                 }
             }
         } else if (warp == 2) {
             // ---------------- packed words (weights: read before the previous kernel ends) ----------------
             Ring<C::kWords> q;
             bool ok = true;
-            for (int t = t0; t < ntiles && ok; t += tstep) {
-                const Tile ti = tile_of<MT>(p, first, t, rank);
-                const int row0 = (ti.expert * G + g0) * int4::kWordsPerGroup;
-                for (int x = 0; x < 2 * ng; ++x, q.advance()) {
+            for (int k = 0; k < sched.items && ok; ++k) {
+                const Tile ti = tile_of<MT>(p, first, sched, k, rank);
+                const int row0 = (ti.expert * G + ti.g0) * int4::kWordsPerGroup;
+                for (int x = 0; x < 2 * ti.ng; ++x, q.advance()) {
                     if (!tc::mbar_wait(&words_empty[q.i], q.parity ^ 1u)) {
                         ok = false;
                         break;
@@ -492,8 +520,9 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
         q.advance(team);
         bool ok = true;
         int x = team;  // steps over all tiles; each team takes every NT-th
-        for (int t = t0; t < ntiles && ok; t += tstep) {
-            for (; x < 2 * ng; x += C::NT, qw.advance(C::NT), q.advance(C::NT)) {
+        for (int k = 0; k < sched.items && ok; ++k) {
+            const Tile ti = tile_of<MT>(p, first, sched, k, rank);
+            for (; x < 2 * ti.ng; x += C::NT, qw.advance(C::NT), q.advance(C::NT)) {
                 if (!tc::mbar_wait(&words_full[qw.i], qw.parity)) {
                     ok = false;
                     break;
@@ -521,7 +550,7 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
                 }
                 __syncwarp();
             }
-            x -= 2 * ng;
+            x -= 2 * ti.ng;
         }
     } else {
         // ---------------- promotion and epilogue ----------------
@@ -532,34 +561,34 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
         constexpr int kLd = MT == 32 ? 16 : 32;  // accumulator columns per round of loads
         uint16_t sc[kAhead];
         const uint16_t *sp = nullptr;
-        auto scales_of = [&](int t) {
-            const Tile ti = tile_of<MT>(p, first, t, rank);
+        auto scales_of = [&](int k) {
+            const Tile ti = tile_of<MT>(p, first, sched, k, rank);
             const int n = ti.n0 + col;
-            sp = p.S + ((size_t)ti.expert * G + g0) * p.N + (n < p.N ? n : 0);
+            sp = p.S + ((size_t)ti.expert * G + ti.g0) * p.N + (n < p.N ? n : 0);
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) sc[k] = __ldg(sp + (size_t)min(k, ng - 1) * p.N);
+            for (int j = 0; j < kAhead; ++j) sc[j] = __ldg(sp + (size_t)min(j, ti.ng - 1) * p.N);
         };
-        if (t0 < ntiles) scales_of(t0);
+        if (sched.items > 0) scales_of(0);
         Ring<C::kAccBufs> b;
         bool ok = true;  // (a warp whose wait timed out still meets the others at their barriers)
-        for (int t = t0; t < ntiles; t += tstep) {
-            const Tile ti = tile_of<MT>(p, first, t, rank);
+        for (int k = 0; k < sched.items; ++k) {
+            const Tile ti = tile_of<MT>(p, first, sched, k, rank);
             uint64_t acc[C::kCols / 2];
 #pragma unroll
             for (int j = 0; j < C::kCols / 2; ++j) acc[j] = 0ull;
-            for (int i0 = 0; i0 < ng && ok; i0 += kAhead) {
+            for (int i0 = 0; i0 < ti.ng && ok; i0 += kAhead) {
 #pragma unroll
-                for (int k = 0; k < kAhead; ++k) {
-                    const int i = i0 + k;
-                    if (i >= ng) break;
+                for (int j = 0; j < kAhead; ++j) {
+                    const int i = i0 + j;
+                    if (i >= ti.ng) break;
                     if (!tc::mbar_wait(&acc_full[b.i], b.parity)) {
                         ok = false;
                         break;
                     }
                     tc::fence_after_sync();
-                    const float s1 = DT::tof(sc[k]);
+                    const float s1 = DT::tof(sc[j]);
                     const uint64_t s = pack2(s1, s1);
-                    sc[k] = __ldg(sp + (size_t)min(i + kAhead, ng - 1) * p.N);
+                    sc[j] = __ldg(sp + (size_t)min(i + kAhead, ti.ng - 1) * p.N);
                     const uint32_t taddr = tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(b.i * MT + jbase);
 #pragma unroll
                     for (int c = 0; c < C::kCols; c += kLd) {
@@ -570,8 +599,8 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
                                 tc::tmem_ld<16>(taddr + c + 16, *reinterpret_cast<float(*)[16]>(&v[16]));
                             tc::tmem_wait_ld();
 #pragma unroll
-                            for (int j = 0; j < kLd; j += 2)
-                                acc[(c + j) / 2] = fma2(pack2(v[j], v[j + 1]), s, acc[(c + j) / 2]);
+                            for (int l = 0; l < kLd; l += 2)
+                                acc[(c + l) / 2] = fma2(pack2(v[l], v[l + 1]), s, acc[(c + l) / 2]);
                         }
                     }
                     tc::fence_before_sync();
@@ -581,9 +610,9 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
                     b.advance();
                 }
             }
-            if (!PAIR && p.SK > 1) {
-                // one tile: its sums [rows][128] go into the stages, whose last readers (the MMAs of the
-                // last group) are through, and are joined below
+            if (!PAIR && k == sched.full && sched.split > 1) {
+                // its sums [rows][128] go into the stages, whose last readers (the MMAs of the last
+                // group) are through, and are joined below
                 float *part = reinterpret_cast<float *>(smem);
 #pragma unroll
                 for (int j = 0; j < C::kCols; j += 2) {
@@ -594,7 +623,7 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
                 }
                 break;
             }
-            if (t + tstep < ntiles) scales_of(t + tstep);
+            if (k + 1 < sched.items) scales_of(k + 1);
             pdl_wait();
             // 16 rows at a time through shared memory, so that a thread takes 8 columns of two rows
             // (storing TMEM lanes directly, 2 bytes a lane, took 20,000-31,000 cycles a tile)
@@ -673,20 +702,24 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
         pdl_launch_dependents();
         regs_dec<C::kRegsOther>();  // every warp goes on with the same share
     }
-    if (!PAIR && p.SK > 1) {
-        const Tile ti = tile_of<MT>(p, first, t0, rank);
-        const float *part = reinterpret_cast<const float *>(smem);
+    if (!PAIR && sched.split > 1) {
         __syncthreads();
         gemv::cluster_sync_all();
-        pdl_wait();
-        const int r0 = ti.rows * sk / p.SK, r1 = ti.rows * (sk + 1) / p.SK;
-        for (int x = r0 * BN + tid; x < r1 * BN; x += C::kThreads) {
-            const uint32_t la = tc::smem_addr(part + x);
-            float v = 0.0f;
-            for (int r = 0; r < p.SK; ++r) v += ld_dsmem_f32(la, (uint32_t)r);
-            const int n = ti.n0 + x % BN;
-            const size_t i = (size_t)(ti.m0 + x / BN) * p.N + n;
-            if (n < p.N) store<DT, POSTOP, OUT_F32>(p, i, v, epi_in<DT, POSTOP, OUT_F32>(p.Other, p.Bias, i, n));
+        if (sched.items > sched.full) {
+            pdl_wait();
+            const Tile ti = tile_of<MT>(p, first, sched, sched.full, rank);
+            const float *part = reinterpret_cast<const float *>(smem);
+            // the cluster's CTAs from `base` on share the tile
+            const int sk = sched.index % sched.split, base = (int)(blockIdx.x % p.cluster) - sk;
+            const int r0 = ti.rows * sk / sched.split, r1 = ti.rows * (sk + 1) / sched.split;
+            for (int x = r0 * BN + tid; x < r1 * BN; x += C::kThreads) {
+                const uint32_t la = tc::smem_addr(part + x);
+                float v = 0.0f;
+                for (int r = 0; r < sched.split; ++r) v += gemv::ld_dsmem_f1(la, (uint32_t)(base + r));
+                const int n = ti.n0 + x % BN;
+                const size_t i = (size_t)(ti.m0 + x / BN) * p.N + n;
+                if (n < p.N) store<DT, POSTOP, OUT_F32>(p, i, v, epi_in<DT, POSTOP, OUT_F32>(p.Other, p.Bias, i, n));
+            }
         }
         gemv::cluster_sync_all();  // every CTA's sums stay until all have read them
     }
@@ -697,6 +730,37 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, Plan<MT>::kCtasPerSm)
         tc::fence_after_sync();
         tmem_dealloc<PAIR>(tmem, C::kTmemCols);
     }
+}
+
+// CTAs that fit the GPU at once in clusters of 1 << c (asked once per device and configuration)
+template <int MT>
+int resident(int c, int sms) {
+    using C = Plan<MT>;
+    static std::atomic<int> known[64][4];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sms;
+    int n = known[dev][c].load();
+    if (n == 0) {
+        auto kern = gemm_int4_kernel<MT, F16, 0, false>;
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = 1u << c;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.gridDim = dim3(sms / (1 << c) * (1 << c));
+        cfg.blockDim = dim3(C::kThreads);
+        cfg.dynamicSmemBytes = C::total;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int clusters = 0;
+        if (ensure_smem(kern, C::total) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) != cudaSuccess)
+            clusters = 0;
+        (void)cudaGetLastError();
+        n = clusters > 0 ? std::min(clusters << c, sms) : sms / (1 << c) * (1 << c);
+        known[dev][c].store(n);
+    }
+    return n;
 }
 
 template <int MT>
@@ -710,13 +774,33 @@ cudaError_t launch(const GemvArgs &a, int sms, const int *meta, int E) {
     e = tc::make_map_plain(&mapB, a.B, CU_TENSOR_MAP_DATA_TYPE_INT32, 4, (meta ? E : 1) * (a.K / int4::kRowsPerWord),
                            a.N, kStepK / int4::kRowsPerWord, BN);
     if (e != cudaSuccess) return e;
-    const int strips = (a.N + BN * C::kCtas - 1) / (BN * C::kCtas);
-    const Params p{(const uint16_t *)a.S, a.C, (const uint16_t *)a.Other, a.Bias, a.M, a.N, a.K, a.SK, strips, meta, E};
+    const int strips = (a.N + BN * C::kCtas - 1) / (BN * C::kCtas), G = a.K / kGS;
     // grouped: an upper bound, every expert adds at most one partial tile
     const long long tiles = ((long long)(a.M + MT - 1) / MT + (meta ? E : 0)) * strips;
-    const long long slots = (long long)sms * C::kCtasPerSm / C::kCtas;
-    const int per_tile = C::kPair ? 2 : a.SK;  // CTAs of a cluster
-    const int grid = (int)(a.SK > 1 || tiles < slots ? tiles : slots) * per_tile;
+    // Cluster size: what makes the rounds over the tiles fewest, in sixteenths of a round (a split
+    // tile costs 1/16 more for its join).  Larger clusters leave some SMs out.  Grouped, the tiles are
+    // only counted on the GPU: clusters of 2, which fill it.
+    int cl = C::kPair || meta ? 1 : 0, units = C::kPair ? sms / 2 : sms / 2 * 2;
+    if (!C::kPair && !meta) {
+        long long best = 1LL << 60;
+        for (int c = 0; c < 4; ++c) {
+            const int n = resident<MT>(c, sms), u = (int)std::min<long long>(n, (tiles << c));
+            if (u < (1 << c)) continue;
+            const long long full = tiles / u, left = tiles - full * u;
+            int split = 1;
+            while (2 * split <= (1 << c) && 2 * split * left <= u && 2 * split <= G) split *= 2;
+            const long long cost = 16 * full + (left ? 16 / split + (split > 1) : 0);
+            if (cost < best) {
+                best = cost;
+                cl = c;
+                units = u;
+            }
+        }
+    }
+    const int cluster = 1 << cl;
+    if (C::kPair || meta) units = (int)std::min<long long>(units, (tiles + cluster - 1) / cluster * cluster);
+    else units = (units + cluster - 1) / cluster * cluster;
+    const Params p{(const uint16_t *)a.S, a.C, (const uint16_t *)a.Other, a.Bias, a.M, a.N, a.K, strips, cluster, meta, E};
     return dispatch_epilogue<GemvArgs>(a, [&](auto dt, auto po, auto of) -> cudaError_t {
         using DT = typename decltype(dt)::type;
         auto kern = gemm_int4_kernel<MT, DT, decltype(po)::value, decltype(of)::value>;
@@ -729,15 +813,14 @@ cudaError_t launch(const GemvArgs &a, int sms, const int *meta, int E) {
         }
         cudaError_t err = ensure_smem(kern, C::total);
         if (err != cudaSuccess) return err;
-        return launch_kernel_cluster(kern, dim3(grid), dim3(C::kThreads), (size_t)C::total, a.stream,
-                                     dim3(per_tile, 1, 1),                                     p, mapA, mapB);
+        return launch_kernel_cluster(kern, dim3(units * C::kCtas), dim3(C::kThreads), (size_t)C::total, a.stream,
+                                     dim3(cluster, 1, 1), p, mapA, mapB);
     });
 }
 
 }  // namespace gemm4
 
 cudaError_t int4_gemm_launch(const GemvArgs &a, int sms, const int *meta, int E) {
-    GemvArgs b = a;
     // activation rows per tile: what the rows (grouped: an expert's average) fill
     const long long per = meta ? (a.M + E - 1) / E : a.M;
     int MT = per <= 32 ? 32 : per <= 64 ? 64 : per <= 128 ? 128 : 256;
@@ -748,16 +831,10 @@ cudaError_t int4_gemm_launch(const GemvArgs &a, int sms, const int *meta, int E)
         const long long pair_waves = (2 * pairs + sms - 1) / sms, waves = (singles + sms - 1) / sms;
         if (3 * pair_waves > 2 * waves) MT = 128;
     }
-    // K split over a cluster while the tiles leave SMs without work
-    const long long tiles = strips * ((a.M + MT - 1) / MT);
-    int sk = 1;
-    if (!meta && MT < 256)
-        while (sk < 8 && 2 * sk <= a.K / kGS && tiles * 2 * sk <= sms) sk *= 2;
-    b.SK = sk;
-    return MT == 32    ? gemm4::launch<32>(b, sms, meta, E)
-           : MT == 64  ? gemm4::launch<64>(b, sms, meta, E)
-           : MT == 128 ? gemm4::launch<128>(b, sms, meta, E)
-                       : gemm4::launch<256>(b, sms, meta, E);
+    return MT == 32    ? gemm4::launch<32>(a, sms, meta, E)
+           : MT == 64  ? gemm4::launch<64>(a, sms, meta, E)
+           : MT == 128 ? gemm4::launch<128>(a, sms, meta, E)
+                       : gemm4::launch<256>(a, sms, meta, E);
 }
 
 cudaError_t read_device_error_gemm_int4(unsigned *out, int reset) { return tc::read_tu_error(out, reset); }

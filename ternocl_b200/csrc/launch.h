@@ -220,16 +220,15 @@ struct MoeTopkArgs {
 cudaError_t moe_topk_launch(const MoeTopkArgs &a);
 // int4 GEMV (gemv_int4.cu), GEMM (gemm_int4.cu; grouped with meta) and MoE decode GEMVs
 // (moe_decode_int4.cu)
-size_t int4_gemv_smem(int M, int K, int SK, int warps);
 cudaError_t int4_gemv_launch(const GemvArgs &a);
 cudaError_t int4_gemm_launch(const GemvArgs &a, int sms, const int *meta = nullptr, int E = 0);
 cudaError_t read_device_error_gemm_int4(unsigned *out, int reset);
 cudaError_t moe_decode_gate_up_int4_launch(const int *ids, const void *X, const uint32_t *Bg, const void *Sg,
                                            const uint32_t *Bu, const void *Su, void *H, int G, int N, int K, int topk,
-                                           int E, int dtype, cudaStream_t st);
+                                           int E, int dtype, int sms, cudaStream_t st);
 cudaError_t moe_decode_down_sum_int4_launch(const int *ids, const void *H, const void *RW, const uint32_t *B,
                                             const void *S, void *O, int T, int N, int K, int topk, int E, int dtype,
-                                            cudaStream_t st);
+                                            int sms, cudaStream_t st);
 cudaError_t read_device_error_moe_decode_int4(unsigned *out, int reset);
 // largest M that TERNOCL_ALGO_AUTO gives the int4 GEMV
 constexpr int kInt4GemvMaxM = 8;

@@ -6,20 +6,19 @@
 // with e = ids[g] and every expert's weights stacked: B [E, K/8, N], S [E, K/128, N].
 //
 // A CTA owns 32 columns of one routed row (gate_up: of both matrices, whose dots meet in
-// the CTA for the SwiGLU; down_sum: of one token, its K running over the topk experts) over
-// the whole K; its W warps split the 128-row groups and are summed in warp order.  A warp
-// streams its groups' words (16 rows x 128 bytes) and scales through a ring in shared memory
-// and turns its activations into int8 digit planes, kChunk groups at a time: a chunk has one
-// exponent, and its sums are scaled back into the warp's totals at its end, so the shared
-// memory does not grow with K.  The dots are mma.sync m16n8k32 s8 x s8, three of the eight
-// n-columns being the digit planes of the row.
+// the CTA for the SwiGLU; down_sum: of one token, its K running over the topk experts side by
+// side) over the whole K; its W warps split the 128-row groups, multiply them in the integer
+// form of gemv_int4_core.cuh and are summed in warp order.  A gate_up warp multiplies its
+// groups of both matrices with the same digit planes.
 //
 // An expert id outside [0, E) contributes zero and sets bit 1 of the device error word.
+//
+// Bound by HBM for several tokens and by latency for one.
+// TIMES
 #include <cuda_runtime.h>
 
 #include "common.cuh"
-#include "gemv_common.cuh"
-#include "int4_common.cuh"
+#include "gemv_int4_core.cuh"
 #include "launch.h"
 #include "tc_common.cuh"
 
@@ -28,16 +27,9 @@ namespace ternocl {
 namespace {
 
 constexpr int kCols = 32;
-constexpr int kRowBytes = kCols * 4;
-constexpr int kWordBytes = int4::kWordsPerGroup * kRowBytes;  // 2 KB
-constexpr int kScaleBytes = kCols * 2;
-constexpr int kStageBytes = kWordBytes + kScaleBytes;
-constexpr int kRingBytes = gemv::kStages * kStageBytes;
-constexpr int kChunk = 8;  // groups per digit staging
-// 128 bytes per group; the 16 more put the planes of two neighbouring lanes' rows on the
-// two 16-byte halves of every 32 bytes (conflict-free 16-byte reads)
-constexpr int kPlane = kChunk * 128 + 16;
-
+// Units (a group of a matrix) a warp has on their way.  Two at 128 registers (16 resident warps)
+// measured best: 4 spill, and with 24 warps at 80 registers 2 do.
+constexpr int kAhead = 2;
 enum Mode { kGateUp = 0, kDownSum = 1 };
 
 struct MParams {
@@ -53,203 +45,131 @@ struct MParams {
 template <int MODE>
 constexpr int kMats = MODE == kGateUp ? 2 : 1;
 
-template <int W, int MODE>
-constexpr size_t smem_bytes() {
-    return (size_t)W * (kRingBytes + 3 * kPlane + kMats<MODE> * kCols * 4);
-}
-
 template <int W, int MODE, class DT>
-__global__ void __launch_bounds__(W * 32) moe_decode_int4_kernel(const MParams p) {
+__global__ void __launch_bounds__(W * 32, 16 / W) moe_decode_int4_kernel(const MParams p) {
     constexpr int NM = kMats<MODE>;
-    extern __shared__ __align__(128) char smem[];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int g = lane >> 2, t = lane & 3;
+    extern __shared__ __align__(128) char smem[];  // the warps' planes
+    __shared__ float red[W][NM][kCols];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int z = blockIdx.x / p.strips;  // routed row (gate_up) or token (down_sum)
     const int n0 = (blockIdx.x - z * p.strips) * kCols;
     const int G = p.K / kGS;
-    const int ng = MODE == kGateUp ? 2 * G : p.topk * G;
-    const int wg0 = (int)((long long)ng * warp / W), nwg = (int)((long long)ng * (warp + 1) / W) - wg0;
-    char *ring = smem + warp * kRingBytes;
-    char *planes = smem + W * kRingBytes + warp * 3 * kPlane;
-    float *red = reinterpret_cast<float *>(smem + W * (kRingBytes + 3 * kPlane));  // [W][NM][32]
+    const int all = MODE == kGateUp ? G : p.topk * G;
+    const int g0 = (int)((long long)all * warp / W), ng = (int)((long long)all * (warp + 1) / W) - g0;
+    int4::DigitRows<1, DT> rows;
+    rows.pbytes = int4::plane_bytes((all + W - 1) / W);
+    rows.planes = smem + warp * 3 * rows.pbytes;
 
     pdl_wait();  // ids and activations come from the kernels before
 
-    // group grp -> its matrix (gate_up) or expert slot (down_sum) and its group there
-    auto part = [&](int grp, int &lg) {
-        const int i = grp / G;
-        lg = grp - i * G;
-        return i;
-    };
-    auto expert = [&](int slot) {
-        const int e = p.ids[MODE == kGateUp ? z : z * p.topk + slot];
-        return e >= 0 && e < p.E ? e : -1;
-    };
-    auto act = [&](int grp) -> const uint16_t * {
-        if (MODE == kGateUp) {
-            int lg;
-            part(grp, lg);
-            return p.A + (size_t)(z / p.topk) * p.K + (size_t)lg * kGS;
-        }
-        return p.A + (size_t)z * p.topk * p.K + (size_t)grp * kGS;  // the token's rows side by side
-    };
-
-    const int col = n0 + 4 * (lane & 7);  // N % 16 == 0: 4-column pieces are whole
-    const bool copies = col < p.N;
-    const bool scales = lane < 4 && n0 + 8 * lane < p.N;
-    int issued = 0;
-    auto issue = [&]() {
-        if (issued < nwg) {
-            char *st = ring + (issued & (gemv::kStages - 1)) * kStageBytes;
-            int lg;
-            const int i = part(wg0 + issued, lg);
-            const int e = expert(i);
-            if (e >= 0) {
-                const uint32_t *B = (MODE == kGateUp && i ? p.B1 : p.B0) +
-                                    ((size_t)e * (p.K / int4::kRowsPerWord) + lg * int4::kWordsPerGroup) * p.N;
-                const uint16_t *S = (MODE == kGateUp && i ? p.S1 : p.S0) + ((size_t)e * G + lg) * p.N;
-                if (copies) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const int r = 4 * c + (lane >> 3);
-                        gemv::cp_async16(st + r * kRowBytes + 16 * (lane & 7), B + (size_t)r * p.N + col);
-                    }
-                }
-                if (scales) gemv::cp_async16(st + kWordBytes + 16 * lane, S + n0 + 8 * lane);
-            }
-        }
-        gemv::cp_async_commit();
-        ++issued;
-    };
-#pragma unroll
-    for (int i = 0; i < gemv::kStages - 1; ++i) issue();
-
-    float total[NM][2][4];
+    const uint16_t *a0 = p.A + (size_t)(MODE == kGateUp ? z / p.topk : z * p.topk) * p.K + (size_t)g0 * kGS;
+    float total[NM][4];
 #pragma unroll
     for (int m = 0; m < NM; ++m)
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) total[m][b][c] = 0.0f;
-    const char *bsrc = g < 3 ? planes + g * kPlane + t * 32 : nullptr;
+        for (int j = 0; j < 4; ++j) total[m][j] = 0.0f;
+    // the next kAhead (matrix, group) units are on their way
+    uint4 w[kAhead][4];
+    uint2 sc[kAhead];
+    float factor[kAhead];
     bool bad_id = false;
-
-    for (int c0 = 0; c0 < nwg; c0 += kChunk) {
-        const int nc = min(kChunk, nwg - c0);
-        // ---- the chunk's activations -> digit planes (16 word rows per group) ----
-        uint32_t mx = 0;
-        uint4 v[kChunk / 2];
+    auto expert = [&](int slot) {
+        const int e = p.ids[slot];
+        bad_id |= e < 0 || e >= p.E;
+        return e >= 0 && e < p.E ? e : -1;
+    };
+    const int col = n0 + 4 * (lane >> 2) < p.N ? n0 + 4 * (lane >> 2) : 0;  // (columns behind N are not stored)
+    const size_t row4 = (size_t)4 * p.N;
+    // group lg of expert e's matrix m into slot k
+    auto load = [&](int k, int m, int e, int lg) {
+        const size_t grp = (size_t)e * G + lg;
+        const uint32_t *wp = (m ? p.B1 : p.B0) + (grp * int4::kWordsPerGroup + (lane & 3)) * p.N + col;
 #pragma unroll
-        for (int i = 0; i < kChunk / 2; ++i) {
-            const int u = 32 * i + lane;  // word row of the chunk
-            v[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (u < 16 * nc) v[i] = __ldg(reinterpret_cast<const uint4 *>(act(wg0 + c0 + u / 16) + 8 * (u % 16)));
-            mx = max(mx, int4::absmax_bits(v[i]));
-        }
-        mx = __reduce_max_sync(0xffffffffu, mx);
-        const int e = digit::exponent_for<DT>(mx);
-        const float rs = int4::inverse_scale<DT>(mx, e);
-        __syncwarp();  // the previous chunk's planes have been read
+        for (int c = 0; c < 4; ++c) w[k][c] = ldg_stream128(wp + c * row4);
+        sc[k] = ldg_stream64((m ? p.S1 : p.S0) + grp * p.N + col);
+    };
+    if constexpr (MODE == kGateUp) {
+        const int e = expert(z);
+        for (int c0 = 0; c0 < ng && e >= 0; c0 += int4::kStage) {
+            const int nc = min(int4::kStage, ng - c0);
+            // unit u: group u / 2 of the stage, of the gate (u even) or the up matrix
+            auto unit = [&](int k, int u) {
+                if (u < 2 * nc) load(k, k & 1, e, g0 + c0 + (u >> 1));
+            };
 #pragma unroll
-        for (int i = 0; i < kChunk / 2; ++i) {
-            const int u = 32 * i + lane;
-            if (u < 16 * nc) {
-                uint2 d[3];
-                int4::word_digits<DT>(v[i], e, d);
-                char *dst = planes + (u / 16) * 128 + (u & 3) * 32 + ((u >> 2) & 3) * 8;
+            for (int k = 0; k < kAhead; ++k) unit(k, k);
+            rows.stage(a0 + (size_t)c0 * kGS, 0, nc, lane);
+            float acc[2][2][4];
 #pragma unroll
-                for (int k = 0; k < 3; ++k) *reinterpret_cast<uint2 *>(dst + k * kPlane) = d[k];
-            }
-        }
-        __syncwarp();
-
-        float acc[NM][2][4];
-#pragma unroll
-        for (int m = 0; m < NM; ++m)
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) acc[m][b][c] = 0.0f;
-
-        for (int i = c0; i < c0 + nc; ++i) {
-            gemv::cp_async_wait<gemv::kStages - 2>();
-            __syncwarp();  // the lanes' copies of this stage are visible to the whole warp
-            const char *st = ring + (i & (gemv::kStages - 1)) * kStageBytes;
-            int lg;
-            const int slot = part(wg0 + i, lg);
-            const int ex = expert(slot);
-            bad_id |= ex < 0;
-            if (ex >= 0) {
-                float gf = 1.0f;
-                if (MODE == kDownSum) gf = DT::tof(p.RW[z * p.topk + slot]);
-                int32_t d[2][4];
+            for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) d[b][c] = (int32_t)digit::kMagicBits;
+                    for (int c = 0; c < 4; ++c) acc[m][b][c] = 0.0f;
+            for (int u0 = 0; u0 < 2 * nc; u0 += kAhead)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint4 b = make_uint4(0u, 0u, 0u, 0u);
-                    if (bsrc) b = *reinterpret_cast<const uint4 *>(bsrc + (i - c0) * 128 + 16 * h);
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const uint4 w = *reinterpret_cast<const uint4 *>(st + (8 * h + 4 * q + t) * kRowBytes + 16 * g);
-                        const uint32_t be = q ? b.z : b.x, bo = q ? b.w : b.y;
-                        int4::imma(d[0], int4::even_rows(w.x), int4::even_rows(w.y), int4::odd_rows(w.x),
-                                   int4::odd_rows(w.y), be, bo);
-                        int4::imma(d[1], int4::even_rows(w.z), int4::even_rows(w.w), int4::odd_rows(w.z),
-                                   int4::odd_rows(w.w), be, bo);
-                    }
+                for (int k = 0; k < kAhead; ++k) {
+                    if (u0 + k >= 2 * nc) break;
+                    rows.group(w[k], sc[k], 1.0f, (u0 + k) >> 1, lane, acc[k & 1]);
+                    unit(k, u0 + k + kAhead);
                 }
-                const uint2 s4 = *reinterpret_cast<const uint2 *>(st + kWordBytes + 8 * g);
-                const float s[4] = {DT::tof((uint16_t)(s4.x & 0xFFFFu)) * gf, DT::tof((uint16_t)(s4.x >> 16)) * gf,
-                                    DT::tof((uint16_t)(s4.y & 0xFFFFu)) * gf, DT::tof((uint16_t)(s4.y >> 16)) * gf};
-#pragma unroll
-                for (int m = 0; m < NM; ++m) {
-                    if (NM > 1 && m != slot) continue;
-#pragma unroll
-                    for (int b = 0; b < 2; ++b)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-                            acc[m][b][c] =
-                                fmaf(__int_as_float(d[b][c]) - digit::kMagic, s[2 * b + (c >> 1)], acc[m][b][c]);
-                }
-            }
-            __syncwarp();  // every lane is done with this stage before it is refilled
-            issue();
+            rows.finish(acc[0], lane, total[0]);
+            rows.finish(acc[1], lane, total[NM - 1]);
         }
+    } else {
+        // the token's experts side by side: a group's expert changes every G groups
+        int lg = g0 % G, slot = z * p.topk + g0 / G, e = ng > 0 ? expert(slot) : -1;
+        float f = ng > 0 ? DT::tof(p.RW[slot]) : 0.0f;
+        for (int c0 = 0; c0 < ng; c0 += int4::kStage) {
+            const int nc = min(int4::kStage, ng - c0);
+            auto unit = [&](int k, int u) {
+                if (u >= nc) return;
+                if (lg == G) {
+                    lg = 0;
+                    ++slot;
+                    e = expert(slot);
+                    f = DT::tof(p.RW[slot]);
+                }
+                factor[k] = f;
+                if (e >= 0) {
+                    load(k, 0, e, lg);
+                } else {  // contributes zero
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) w[k][c] = make_uint4(0u, 0u, 0u, 0u);
+                    sc[k] = make_uint2(0u, 0u);
+                    factor[k] = 0.0f;
+                }
+                ++lg;
+            };
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) unit(k, k);
+            rows.stage(a0 + (size_t)c0 * kGS, 0, nc, lane);
+            float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            for (int u0 = 0; u0 < nc; u0 += kAhead)
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    if (u0 + k >= nc) break;
+                    rows.group(w[k], sc[k], factor[k], u0 + k, lane, acc);
+                    unit(k, u0 + k + kAhead);
+                }
+            rows.finish(acc, lane, total[0]);
+        }
+    }
+    if ((lane & 3) == 0) {
 #pragma unroll
         for (int m = 0; m < NM; ++m)
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) total[m][b][c] = fmaf(acc[m][b][c], rs, total[m][b][c]);
+            *reinterpret_cast<float4 *>(&red[warp][m][lane]) =
+                make_float4(total[m][0], total[m][1], total[m][2], total[m][3]);
     }
-    gemv::cp_async_wait<0>();
     if (bad_id && lane == 0) atomicOr(&tc::g_device_error, 2u);
     pdl_launch_dependents();
-    __syncwarp();
-
-    // ---- digit planes -> column values of this warp: tb[mat][plane][col] in its ring ----
-    float(*tb)[8][kCols] = reinterpret_cast<float(*)[8][kCols]>(ring);
-#pragma unroll
-    for (int m = 0; m < NM; ++m)
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tb[m][2 * t + (c & 1)][4 * g + 2 * b + (c >> 1)] = total[m][b][c];
-    __syncwarp();
-#pragma unroll
-    for (int m = 0; m < NM; ++m)
-        red[(warp * NM + m) * kCols + lane] =
-            (tb[m][0][lane] + 256.0f * tb[m][1][lane]) + 65536.0f * tb[m][2][lane];
     __syncthreads();
     if (warp != 0) return;
     float v[NM];
 #pragma unroll
     for (int m = 0; m < NM; ++m) {
         v[m] = 0.0f;
-        for (int w = 0; w < W; ++w) v[m] += red[(w * NM + m) * kCols + lane];
+        for (int w = 0; w < W; ++w) v[m] += red[w][m][lane];
     }
     const int n = n0 + lane;
     if (n < p.N) p.out[(size_t)z * p.N + n] = DT::fromf(MODE == kGateUp ? epi<1>(v[0], v[NM - 1]) : v[0]);
@@ -258,36 +178,41 @@ __global__ void __launch_bounds__(W * 32) moe_decode_int4_kernel(const MParams p
 template <int W, int MODE, class DT>
 cudaError_t launch_w(const MParams &p, int rows, cudaStream_t st) {
     auto kern = moe_decode_int4_kernel<W, MODE, DT>;
-    constexpr size_t smem = smem_bytes<W, MODE>();
-    cudaError_t e = ensure_smem(kern, smem);
+    const int all = (MODE == kGateUp ? 1 : p.topk) * (p.K / kGS);
+    const size_t smem = (size_t)W * 3 * int4::plane_bytes((all + W - 1) / W);  // <= 50 KB
+    const cudaError_t e = ensure_smem(kern, smem);
     if (e != cudaSuccess) return e;
     return launch_kernel(kern, dim3((unsigned)p.strips * (unsigned)rows), dim3(W * 32), smem, st, p);
 }
 
+// 8 warps split K while the CTAs fill the SMs less than twice, else 4, whose longer ranges spend
+// less on their ends: gate_up (K 2048, N 768, top-8) 1 token 5.9 against 7.3 us, 2 tokens 10.2
+// against 9.1, 9 tokens 29.4 against 25.4; down_sum 4 tokens 9.1 against 11.7, 9 tokens 16.4
+// against 15.4.
 template <int MODE>
-cudaError_t launch(const MParams &p, int rows, int dtype, cudaStream_t st) {
-    const int ng = (MODE == kGateUp ? 2 : p.topk) * (p.K / kGS);
+cudaError_t launch(const MParams &p, int rows, int sms, int dtype, cudaStream_t st) {
+    const bool many = (long long)rows * p.strips >= 2LL * sms;
     if (dtype == TERNOCL_BF16)
-        return ng >= 16 ? launch_w<8, MODE, BF16>(p, rows, st) : launch_w<4, MODE, BF16>(p, rows, st);
-    return ng >= 16 ? launch_w<8, MODE, F16>(p, rows, st) : launch_w<4, MODE, F16>(p, rows, st);
+        return many ? launch_w<4, MODE, BF16>(p, rows, st) : launch_w<8, MODE, BF16>(p, rows, st);
+    return many ? launch_w<4, MODE, F16>(p, rows, st) : launch_w<8, MODE, F16>(p, rows, st);
 }
 
 }  // namespace
 
 cudaError_t moe_decode_gate_up_int4_launch(const int *ids, const void *X, const uint32_t *Bg, const void *Sg,
                                            const uint32_t *Bu, const void *Su, void *H, int G, int N, int K, int topk,
-                                           int E, int dtype, cudaStream_t st) {
+                                           int E, int dtype, int sms, cudaStream_t st) {
     const MParams p{ids, (const uint16_t *)X, Bg, Bu, (const uint16_t *)Sg, (const uint16_t *)Su, nullptr,
                     (uint16_t *)H, N, K, topk, E, (N + kCols - 1) / kCols};
-    return launch<kGateUp>(p, G, dtype, st);
+    return launch<kGateUp>(p, G, sms, dtype, st);
 }
 
 cudaError_t moe_decode_down_sum_int4_launch(const int *ids, const void *H, const void *RW, const uint32_t *B,
                                             const void *S, void *O, int T, int N, int K, int topk, int E, int dtype,
-                                            cudaStream_t st) {
+                                            int sms, cudaStream_t st) {
     const MParams p{ids, (const uint16_t *)H, B, B, (const uint16_t *)S, (const uint16_t *)S, (const uint16_t *)RW,
                     (uint16_t *)O, N, K, topk, E, (N + kCols - 1) / kCols};
-    return launch<kDownSum>(p, T, dtype, st);
+    return launch<kDownSum>(p, T, sms, dtype, st);
 }
 
 cudaError_t read_device_error_moe_decode_int4(unsigned *out, int reset) { return tc::read_tu_error(out, reset); }
