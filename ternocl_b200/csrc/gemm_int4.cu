@@ -20,7 +20,7 @@
 //   warp 1      the MMA issuer (of a pair: the first CTA's): per step 4 tcgen05.mma kind::f16
 //               (M=128 a CTA, N=rows rounded up, K=16) into one of kAccBufs accumulators;
 //   warp 2      the packed words of a step: one TMA box of 8 word rows x 128 columns;
-//   warp 3      TMEM allocation;
+//   warp 3      TMEM allocation, and with few rows the MMAs of every other group;
 //   4 NT warps  decode, NT teams of 4 that take the steps in turn: one lane makes one 8 x 8 core
 //               matrix of the M operand (MN-major) out of 8 words;
 //   NP warps    promotion: tcgen05.ld of a finished group, acc += S * D_g (f32x2), and at the
@@ -66,28 +66,34 @@ constexpr int kOutRow = BN + 16, kOutRows = 8, kOutBytes = kOutRows * kOutRow * 
 
 // Threads, rings and register shares by the rows of a tile; one CTA per SM.  kRegs*: setmaxnreg
 // values (0: not used), whose sum over the warps stays within what the block launches with.
-// Few rows leave shared memory for words: 64 to 80 KB of them on their way cover the ~1.2 us
-// that they take from HBM.
+// Few rows leave shared memory for words, to cover the ~1.2 us that they take from HBM, and two
+// MMA issuers, since a step's MMAs then take less than the ~330 cycles that one issuer spends on it.
+//
+// A wait for a barrier's parity tells a pass from the one before only for a role that sees every
+// pass of the slot, or whose earlier waits imply the pass before.  One issuer does the steps in
+// order, so a decode team at step x, which has waited for step x - NT's slot, knows that step
+// x - 2 kSteps is done if NT <= kSteps.  Two issuers do not, so there every slot has one team
+// and one issuer: kSteps and kWords are multiples of NT and kSteps of 4.
 template <int MT_>
 struct Cfg;
 template <>
 struct Cfg<256> {
-    static constexpr int MT = 256, NT = 2, NP = 8, kSteps = 5, kWords = 6, kAccBufs = 2;
+    static constexpr int MT = 256, NT = 2, NP = 8, kSteps = 5, kWords = 6, kAccBufs = 2, kIssuers = 1;
     static constexpr int kRegsPromote = 168, kRegsOther = 48;
 };
 template <>
 struct Cfg<128> {
-    static constexpr int MT = 128, NT = 3, NP = 8, kSteps = 4, kWords = 16, kAccBufs = 4;
+    static constexpr int MT = 128, NT = 3, NP = 8, kSteps = 4, kWords = 16, kAccBufs = 4, kIssuers = 1;
     static constexpr int kRegsPromote = 112, kRegsOther = 64;
 };
 template <>
 struct Cfg<64> {
-    static constexpr int MT = 64, NT = 4, NP = 4, kSteps = 5, kWords = 20, kAccBufs = 4;
+    static constexpr int MT = 64, NT = 4, NP = 4, kSteps = 4, kWords = 28, kAccBufs = 4, kIssuers = 2;
     static constexpr int kRegsPromote = 112, kRegsOther = 72;
 };
 template <>
 struct Cfg<32> {
-    static constexpr int MT = 32, NT = 4, NP = 4, kSteps = 6, kWords = 20, kAccBufs = 4;
+    static constexpr int MT = 32, NT = 4, NP = 4, kSteps = 8, kWords = 12, kAccBufs = 4, kIssuers = 2;
     static constexpr int kRegsPromote = 0, kRegsOther = 0;
 };
 
@@ -111,15 +117,18 @@ struct Plan : Cfg<MT> {
     static constexpr int dec = a + C::kSteps * kABytes;
     static constexpr int words = dec + C::kSteps * kDecBytes;
     static constexpr int bars = words + C::kWords * kWordBytes;
-    static constexpr int first = bars + 512;  // grouped: first tile of every expert
+    static constexpr int first = bars + 640;  // grouped: first tile of every expert
     // the epilogue's blocks: two of 8 rows for every 4 promotion warps
     static constexpr int out = (first + (kMaxExperts + 1) * 4 + 15) / 16 * 16;
     static constexpr int total = out + C::NP / 4 * 2 * kOutBytes + 1024;  // + alignment slack
     static_assert(total <= 227 * 1024, "shared memory");
     static_assert(kPair || MT * BN * 4 <= words, "the split's sums reuse the stages");
     static_assert(C::NT <= C::kSteps && C::NT <= C::kWords, "decode teams");
+    static_assert(C::kIssuers == 1 || (C::kSteps % C::NT == 0 && C::kWords % C::NT == 0 && C::kSteps % 4 == 0 &&
+                                       C::kAccBufs % 2 == 0),
+                  "two issuers: a slot belongs to one team and one issuer");
     static_assert(kTmemCols <= 512 && (kTmemCols & (kTmemCols - 1)) == 0, "TMEM");
-    static_assert((2 * C::kSteps + 2 * C::kWords + 2 * C::kAccBufs) * 8 + 4 <= 512, "barriers");
+    static_assert((2 * C::kSteps + 2 * C::kWords + 2 * C::kAccBufs) * 8 + 4 <= 640, "barriers");
 };
 
 struct Params {
@@ -438,19 +447,22 @@ __global__ void __launch_bounds__(Plan<MT>::kThreads, 1)
                     tc::mbar_wait(&ready[q.i], q.parity ^ 1u);
                 }
             }
-        } else if (warp == 1 && rank == 0) {
+        } else if ((warp == 1 || (C::kIssuers == 2 && warp == 3)) && rank == 0) {
             // ---------------- MMA issuer ----------------
-            // (one: a decode team waits for the parity of the last pass over its slot, which tells that
-            // pass from the one before only while the steps are done in order and NT <= kSteps)
             Ring<C::kSteps> q;
             Ring<C::kAccBufs> b;
             bool ok = true;
+            int c = 0;  // groups over all tiles
             for (int k = 0; k < sched.items && ok; ++k) {
                 const Tile ti = tile_of<MT>(p, first, sched, k, rank);
                 // M operand MN-major (bit 15), N operand K-major
                 const int nrows = PAIR ? (ti.rows + 31) & ~31 : (ti.rows + 15) & ~15;
                 const uint32_t idesc = tc::idesc_f16(DT::kBF16, BN * C::kCtas, nrows) | (1u << 15);
-                for (int i = 0; i < ti.ng && ok; ++i, b.advance()) {
+                for (int i = 0; i < ti.ng && ok; ++i, ++c, b.advance()) {
+                    if (C::kIssuers == 2 && (c & 1) != (warp >> 1)) {
+                        q.advance(2);
+                        continue;
+                    }
                     if (!tc::mbar_wait(&acc_empty[b.i], b.parity ^ 1u)) {
                         ok = false;
                         break;
