@@ -378,23 +378,31 @@ def _raw_stream(device):
     return get(device) if get is not None else torch.cuda.current_stream(device).cuda_stream
 
 
+_ENTRIES = {}
+
+
 def _launch(name, like, stream, *args):
     """Call entry point `name` on `like`'s device (made current for the call if it is not); no rows, no call."""
-    torch = _torch()
     if like.shape[0] == 0:
         return
+    entry = _ENTRIES.get(name)
+    if entry is None:
+        entry = _ENTRIES.setdefault(name, getattr(lib(), name))
+    torch = _torch()
     device = like.get_device()
     s = _raw_stream(device) if stream is None else _stream(stream)
     if device == torch.cuda.current_device():
-        call(name, *args, s)
+        status = entry(*args, s)
     else:
         with torch.cuda.device(device):
-            call(name, *args, s)
+            status = entry(*args, s)
+    if status:
+        raise TernoclError(name, status)
 
 
 def _expect(name, t, shape, dtype, like):
     """`t` is a contiguous CUDA tensor of this shape and dtype on `like`'s device."""
-    if t.is_cuda and t.get_device() == like.get_device() and t.shape == shape and t.dtype == dtype and t.is_contiguous():
+    if t.shape == shape and t.dtype == dtype and t.get_device() == like.get_device() >= 0 and t.is_contiguous():
         return
     if not t.is_cuda or not t.is_contiguous() or t.device != like.device:
         raise ValueError("%s must be a contiguous CUDA tensor on %s" % (name, like.device))
@@ -411,11 +419,12 @@ def _expect_int4(name, B, S, lead, K, N, like):
 
 
 def _rows2(name, A):
-    if A.dim() != 2:
-        raise ValueError("%s must be [rows, K], got %s" % (name, tuple(A.shape)))
-    _expect(name, A, A.shape, A.dtype, A)
-    M, K = A.shape
-    return dtype_code(A), M, K
+    shape = A.shape
+    if len(shape) != 2:
+        raise ValueError("%s must be [rows, K], got %s" % (name, tuple(shape)))
+    if not A.is_cuda or not A.is_contiguous():
+        raise ValueError("%s must be a contiguous CUDA tensor" % name)
+    return dtype_code(A), shape[0], shape[1]
 
 
 def _result(out, shape, dtype, like):
@@ -428,7 +437,7 @@ def _result(out, shape, dtype, like):
 def _int4_epilogue(A, M, N, postop, out_f32, other, bias):
     """Checks the epilogue's operands; the output's dtype."""
     dtype = _torch().float32 if out_f32 else A.dtype
-    if postop in (POSTOP_SILU_MUL, POSTOP_ADD):
+    if postop == POSTOP_SILU_MUL or postop == POSTOP_ADD:
         if other is None:
             raise ValueError("postop %d needs other" % postop)
         _expect("other", other, (M, N), A.dtype, A)
@@ -535,8 +544,10 @@ def moe_topk(logits, topk, bias=None, scoring="softmax", n_group=1, topk_group=1
         raise ValueError("scoring must be 'softmax' or 'sigmoid', got %r" % (scoring,))
     if logits.dim() != 2 or logits.dtype not in codes:
         raise TypeError("logits must be [T, E] in fp32, fp16 or bf16")
-    _expect("logits", logits, logits.shape, logits.dtype, logits)
+    if not logits.is_cuda or not logits.is_contiguous():
+        raise ValueError("logits must be a contiguous CUDA tensor")
     T, E = logits.shape
+    topk = int(topk)
     if dtype is None:
         dtype = logits.dtype if out is None else out.dtype
     if dtype not in codes:
@@ -544,11 +555,11 @@ def moe_topk(logits, topk, bias=None, scoring="softmax", n_group=1, topk_group=1
     if bias is not None:
         _expect("bias", bias, (E,), torch.float32, logits)
     if ids is None:
-        ids = logits.new_empty((T, int(topk)), dtype=torch.int32)
+        ids = logits.new_empty((T, topk), dtype=torch.int32)
     else:
-        _expect("ids", ids, (T, int(topk)), torch.int32, logits)
-    RW = _result(out, (T, int(topk)), dtype, logits)
-    _launch("ternocl_moe_topk", logits, stream, _ptr(logits), _ptr(bias), _ptr(ids), _ptr(RW), T, E, int(topk),
+        _expect("ids", ids, (T, topk), torch.int32, logits)
+    RW = _result(out, (T, topk), dtype, logits)
+    _launch("ternocl_moe_topk", logits, stream, _ptr(logits), _ptr(bias), _ptr(ids), _ptr(RW), T, E, topk,
             SCORE_SOFTMAX if scoring == "softmax" else SCORE_SIGMOID, int(n_group), int(topk_group), int(group_top),
             int(bool(renormalize)), float(scale), codes[logits.dtype], codes[dtype])
     return ids, RW

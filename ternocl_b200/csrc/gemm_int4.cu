@@ -835,6 +835,10 @@ cudaError_t launch(const GemvArgs &a, int sms, const int *meta, int E) {
 cudaError_t int4_gemm_launch(const GemvArgs &a, int sms, const int *meta, int E) {
     // activation rows per tile: what the rows (grouped: an expert's average) fill
     const long long per = meta ? (a.M + E - 1) / E : a.M;
+    // Up to 24 rows by gemm_int4_rows.cu where its 256-column tiles, split 8 ways, fill the SMs: 5376x21504
+    // at M = 16 23.5 against 31.6 us here, at M = 24 28.5 against 33.0; 4096x6144 at M = 16 10.9 against 12.5;
+    // 14336x4096 at M = 16 23.4 against 17.2.
+    if (!meta && a.M <= kInt4RowsMaxM && (long long)((a.N + 255) / 256) * 8 >= sms) return int4_rows_launch(a, sms);
     int MT = per <= 32 ? 32 : per <= 64 ? 64 : per <= 128 ? 128 : 256;
     const long long strips = (a.N + gemm4::BN - 1) / gemm4::BN;
     if (MT == 256 && !meta) {

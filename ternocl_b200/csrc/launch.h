@@ -222,6 +222,9 @@ cudaError_t moe_topk_launch(const MoeTopkArgs &a);
 // (moe_decode_int4.cu)
 cudaError_t int4_gemv_launch(const GemvArgs &a);
 cudaError_t int4_gemm_launch(const GemvArgs &a, int sms, const int *meta = nullptr, int E = 0);
+// the int4 product for up to kInt4RowsMaxM rows (gemm_int4_rows.cu)
+constexpr int kInt4RowsMaxM = 24;
+cudaError_t int4_rows_launch(const GemvArgs &a, int sms);
 cudaError_t read_device_error_gemm_int4(unsigned *out, int reset);
 cudaError_t moe_decode_gate_up_int4_launch(const int *ids, const void *X, const uint32_t *Bg, const void *Sg,
                                            const uint32_t *Bu, const void *Su, void *H, int G, int N, int K, int topk,
