@@ -348,3 +348,92 @@ def test_custom_operators(cuda, tl):
     for op, args in ((torch.ops.ternocl.int4_linear.default, (A, B, S)),
                      (torch.ops.ternocl.moe_topk.default, (logits, 4))):
         torch.library.opcheck(op, args, test_utils=("test_schema", "test_faketensor"))
+
+
+# ------------------------------------------------------------- every kernel and schedule of the linear layer
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("M,K,N", [
+    (9, 128, 4864), (16, 640, 5008), (17, 256, 4880), (24, 1280, 9232),  # 9 to 24 rows, many columns
+    (25, 640, 19216), (64, 1280, 19200), (40, 256, 38416),               # a full round of tiles and a split one
+    (100, 384, 19216), (300, 256, 19344),
+    (512, 640, 8208), (700, 384, 16400), (257, 1152, 37904),             # CTA pairs, odd strips among them
+    (1, 17408, 7136), (2, 17408, 7136), (8, 4096, 7136)])                # long ranges per warp
+def test_linear_kernels(cuda, tl, bf16, M, K, N):
+    linear_case(tl, M + K + N, M, K, N, bf16, 2 if M % 2 else 1, bool(K & 128), 0)
+    assert tl.device_error() == 0
+
+
+@pytest.mark.parametrize("M", [9, 20])
+@pytest.mark.parametrize("postop", [0, 1, 2, 3, 4])
+@pytest.mark.parametrize("out_f32", [False, True])
+def test_linear_epilogues_of_few_rows(cuda, tl, M, postop, out_f32):
+    linear_case(tl, M + postop, M, 384, 4912, postop & 1, postop, out_f32, 0)
+    linear_case(tl, M + postop, 30 * M, 256, 16400, postop & 1, postop, out_f32, 0)
+    assert tl.device_error() == 0
+
+
+def test_linear_calls_on_two_streams_at_once(cuda, tl):
+    """Nothing is shared between calls that overlap: the same results as one after the other."""
+    g = gen(13)
+    cases = []
+    for M, K, N in ((1, 4096, 8192), (16, 1024, 8192), (64, 1024, 4096), (600, 512, 8192)):
+        B, S = weights(g, K, N, dtype=torch.float16)
+        cases.append((activations(g, M, K, torch.float16), B, (S / K ** 0.5).half()))
+    want = [tl.int4_upcvt(*c) for c in cases]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(4):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k] += [tl.int4_upcvt(*c) for c in (cases if k else cases[::-1])]
+    torch.cuda.synchronize()
+    for k in range(2):
+        for i, C in enumerate(got[k]):
+            assert torch.equal(C, want[i % 4 if k else 3 - i % 4])
+    assert tl.device_error() == 0
+
+
+def test_linear_residual_in_place(cuda, tl):
+    """C may be Other itself (the residual's own buffer)."""
+    g = gen(14)
+    for M, N in ((1, 512), (6, 512), (16, 5120), (40, 512), (300, 8192)):
+        A = activations(g, M, 512, torch.bfloat16)
+        B, S = weights(g, 512, N, dtype=torch.bfloat16)
+        x = torch.randn(M, N, generator=g, device="cuda").bfloat16()
+        want = tl.int4_upcvt(A, B, S, postop=2, other=x)
+        tl.int4_upcvt(A, B, S, postop=2, other=x, out=x)
+        assert torch.equal(x, want), (M, N)
+
+
+def test_functions_refuse_what_does_not_fit(cuda, tl):
+    g = gen(15)
+    B, S = weights(g, 256, 64, dtype=torch.float16)
+    A = activations(g, 2, 256, torch.float16)
+    ok = tl.int4_upcvt(A, B, S)
+    for bad in (dict(A=A.float()), dict(A=A[:, :128].contiguous()), dict(A=A.t()), dict(B=B.long()), dict(B=B[:-1]),
+                dict(B=B[:, ::2]), dict(S=S.bfloat16()), dict(S=S[:1]), dict(S=S.cpu()), dict(A=A[0])):
+        with pytest.raises((ValueError, TypeError, IndexError)):
+            tl.int4_upcvt(**{"A": A, "B": B, "S": S, **bad})
+    for bad in (dict(postop=1), dict(postop=2, other=ok.float()), dict(postop=2, other=ok[:1]), dict(postop=3),
+                dict(postop=3, bias=ok[0].float()), dict(out=ok.float()), dict(out=ok[:1]), dict(out_f32=True, out=ok)):
+        with pytest.raises((ValueError, TypeError)):
+            tl.int4_upcvt(A, B, S, **bad)
+    with pytest.raises(tl.TernoclError):
+        tl.int4_upcvt(A, B, S, postop=7)
+    buf = torch.zeros(2 * 64 + 4, dtype=torch.float16, device="cuda")
+    with pytest.raises(tl.TernoclError):  # 8-byte aligned only
+        tl.int4_upcvt(A, B, S, out=buf[4:132].view(2, 64))
+    ids = torch.zeros(4, dtype=torch.int32, device="cuda")
+    Be, Se = B[None], S[None]
+    with pytest.raises(ValueError):
+        tl.moe_decode_gate_up_int4(ids[:3], A, Be, Se, Be, Se, 1, 2)
+    with pytest.raises(ValueError):
+        tl.moe_decode_gate_up_int4(ids, A, Be, Se, Be, Se, 2, 2)
+    with pytest.raises(ValueError):
+        tl.moe_decode_down_sum_int4(ids[:2], A, torch.ones(3, device="cuda").half(), Be, Se, 1, 2)
+    with pytest.raises(ValueError):
+        tl.moe_gemm_int4(ids, A, Be, Se, 2)
+    with pytest.raises(tl.TernoclError):
+        tl.moe_gemm_int4(ids, A, Be, Se, 1, postop=3)
