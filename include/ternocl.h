@@ -354,7 +354,10 @@ int ternocl_moe_decode_down_sum(const int32_t *ids, const void *H, const void *R
  * values that are not finite or not meaningful in that row of C only.
  *
  * Linear layer:  C[m,n] = DT(epi( sum_k A[m,k] * code(B[k,n]) * S[k/128, n] )).
- * algo: GEMV (decode), GEMM (tcgen05), or AUTO (the GEMV up to M = 8).  No workspace: a K
+ * algo: GEMV (decode, in blocks of 8 rows), GEMM (from 9 rows on: tcgen05, or for up to 24 rows
+ * and many columns warp-level MMAs), or AUTO (the GEMV up to M = 8).  With M <= 2 the GEMV takes
+ * the activations as fixed-point numbers, exact to 2^-23 of the largest of a range of K (and a
+ * row with an Inf or a NaN gives NaN).  No workspace: a K
  * split stays within one thread-block cluster.  M <= 524280; C and Other 16-byte aligned. */
 int ternocl_int4_upcvt(const void *A, const uint32_t *B, const void *S, void *C, const void *Other,
                        const void *Bias, int M, int N, int K, int dtype, int postop, int out_f32, int algo,

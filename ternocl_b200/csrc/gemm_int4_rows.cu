@@ -13,7 +13,8 @@
 // order) are whole rows.
 //
 // Bound by issue: ~180 instructions decode a group of 32 columns, ~55 more per block of 8 rows.
-// TIMES
+// Measured on B200 (bf16, CUDA graph): 5376x21504 M=9 22.7 us, M=16 23.5 us (on the tcgen05 GEMM
+// 31.0 and 31.6), M=24 28.5 us (33.0); floor 9.4 us, the words once.
 #include <cuda_runtime.h>
 
 #include "common.cuh"

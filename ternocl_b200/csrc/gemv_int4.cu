@@ -15,7 +15,11 @@
 // 223 us, 2.9 TB/s).  Reading further ahead (2 to 4 groups at 80 to 128 registers) measured
 // the same or slower, and so did CTAs that walk several strips with the planes kept and the
 // next strip's words on their way (134 against 130 us).
-// TIMES
+// Measured on B200 (bf16, CUDA graph, us; floor = words and scales at 6.45 TB/s): 4096x4096 M=1 4.45
+// (1.3), M=8 5.65; 4096x28672 M=1 17.1 (9.4), M=8 20.2; 5376x21504 M=1 15.6 (9.3), M=8 17.3;
+// 14336x4096 M=1 10.9 (4.7); 5120x248320 M=1 126 (102), M=8 156.  ncu, 5120x124160 M=1
+// (profiles/int4_gemv_gemm.md): DRAM reads = words + scales, issue 54 % busy, 256 instructions
+// per group and warp with a CTA's ends counted in.
 #include <cuda_runtime.h>
 
 #include "gemv_common.cuh"

@@ -13,8 +13,10 @@
 //
 // An expert id outside [0, E) contributes zero and sets bit 1 of the device error word.
 //
-// Bound by HBM for several tokens and by latency for one.
-// TIMES
+// Bound by latency for one token (ids, then words, then one or two groups per warp) and by the
+// many short CTAs for several.  Measured on B200 (K 2048, N 768 and back, 128 experts, top-8, CUDA
+// graph): gate_up 1 token 6.0 us (floor 2.0: every touched expert's words once), 9 tokens 25.4 us
+// (14.2); down_sum 6.0 us (1.0) and 15.4 us (7.1).
 #include <cuda_runtime.h>
 
 #include "common.cuh"
