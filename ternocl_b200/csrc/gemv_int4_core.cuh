@@ -168,27 +168,34 @@ struct DigitRows {
     int pbytes;      // of a plane
     float rs[ROWS];  // what an integer of row m's planes counts
 
-    __device__ __forceinline__ void stage(const uint16_t *a0, size_t a_stride, int ng, int lane) {
+    // `use(group)`: false has that group's activations taken as zeros
+    template <class Use>
+    __device__ __forceinline__ void stage(const uint16_t *a0, size_t a_stride, int ng, int lane, Use use) {
         __syncwarp();  // the planes' last readers are through
 #pragma unroll
         for (int m = 0; m < ROWS; ++m) {
             const uint4 *a = reinterpret_cast<const uint4 *>(a0 + m * a_stride);
             uint32_t mx = 0;
 #pragma unroll 1
-            for (int u = lane; u < 16 * ng; u += 32) mx = max(mx, absmax_bits(__ldg(a + u)));
+            for (int u = lane; u < 16 * ng; u += 32)
+                if (use(u >> 4)) mx = max(mx, absmax_bits(__ldg(a + u)));
             mx = __reduce_max_sync(0xffffffffu, mx);
             const int e = digit::exponent_for<DT>(mx);
             rs[m] = inverse_scale<DT>(mx, e);
 #pragma unroll 1
             for (int u = lane; u < 16 * ng; u += 32) {  // word row u
                 uint2 d[3];
-                word_digits<DT>(__ldg(a + u), e, d);
+                word_digits<DT>(use(u >> 4) ? __ldg(a + u) : make_uint4(0u, 0u, 0u, 0u), e, d);
                 char *dst = planes + 3 * m * pbytes + (u / 16) * 128 + (u & 3) * 32 + ((u >> 2) & 3) * 8;
 #pragma unroll
                 for (int k = 0; k < 3; ++k) *reinterpret_cast<uint2 *>(dst + k * pbytes) = d[k];
             }
         }
         __syncwarp();
+    }
+
+    __device__ __forceinline__ void stage(const uint16_t *a0, size_t a_stride, int ng, int lane) {
+        stage(a0, a_stride, ng, lane, [](int) { return true; });
     }
 
     // acc += (staged group i) x w, scaled by s4 * factor: acc[b][c] is column 4g + 2b + (c >> 1),

@@ -11,7 +11,7 @@
 // form of gemv_int4_core.cuh and are summed in warp order.  A gate_up warp multiplies its
 // groups of both matrices with the same digit planes.
 //
-// An expert id outside [0, E) contributes zero and sets bit 1 of the device error word.
+// An expert id outside [0, E) contributes zero, whatever its activations, and sets bit 1 of the device error word.
 //
 // Bound by latency for one token (ids, then words, then one or two groups per warp) and by the
 // many short CTAs for several.  Measured on B200 (K 2048, N 768 and back, 128 experts, top-8, CUDA
@@ -145,7 +145,14 @@ __global__ void __launch_bounds__(W * 32, 16 / W) moe_decode_int4_kernel(const M
             };
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) unit(k, k);
-            rows.stage(a0 + (size_t)c0 * kGS, 0, nc, lane);
+            // a left-out expert's activations must not reach the others through the planes' common scale
+            const uint16_t *a = a0 + (size_t)c0 * kGS;
+            const int at = g0 + c0, s0 = z * p.topk + at / G, s1 = z * p.topk + (at + nc - 1) / G;
+            auto valid = [&](int s) { return (unsigned)p.ids[s] < (unsigned)p.E; };
+            bool all_valid = true;
+            for (int s = s0; s <= s1; ++s) all_valid &= valid(s);
+            if (all_valid) rows.stage(a, 0, nc, lane);
+            else rows.stage(a, 0, nc, lane, [&](int i) { return valid(z * p.topk + (at + i) / G); });
             float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
             for (int u0 = 0; u0 < nc; u0 += kAhead)
 #pragma unroll

@@ -219,6 +219,25 @@ def test_decode_bad_expert_ids_contribute_zero(cuda, tl):
     assert tl.device_error() == 0
 
 
+@pytest.mark.parametrize("T,topk,K", [(1, 6, 128), (3, 8, 384), (40, 8, 128), (1, 3, 4096)])
+def test_down_sum_ignores_the_activations_of_bad_ids(cuda, tl, T, topk, K):
+    """Left-out rows (another device's experts, say) may hold anything: NaN, Inf, or values so large that
+    sharing a fixed-point scale with them would wipe the others out."""
+    g, E, N = gen(T * K), 5, 144
+    H, ids = activations(g, T * topk, K, torch.bfloat16), torch.randint(0, E, (T * topk,), generator=g, device="cuda",
+                                                                       dtype=torch.int32)
+    B, S = weights(g, E, K, N, dtype=torch.bfloat16)
+    RW = torch.rand(T * topk, generator=g, device="cuda").bfloat16()
+    ids[1::2] = -1
+    H[1::2] = 0
+    want = tl.moe_decode_down_sum_int4(ids, H, RW, B, S, E, topk)
+    assert bool(want.isfinite().all()) and bool(want.any())
+    for v in (float("nan"), float("inf"), 3e38):
+        H[1::2] = v
+        assert torch.equal(tl.moe_decode_down_sum_int4(ids, H, RW, B, S, E, topk), want), v
+    assert tl.device_error(reset=True) == 2
+
+
 @pytest.mark.parametrize("bf16", [0, 1])
 @pytest.mark.parametrize("T,topk,E,K,N,postop,out_f32", [
     (1, 1, 1, 128, 16, 0, True), (5, 2, 4, 256, 144, 1, False), (40, 4, 8, 640, 272, 2, True),
