@@ -208,6 +208,8 @@ def moe_prefill_int4(X: torch.Tensor, ids: torch.Tensor, RW: torch.Tensor, Bg: t
                      topk: int) -> torch.Tensor:
     """moe_prefill with 4-bit experts: B* int32 [E, K/8, N], S* [E, K/128, N]."""
     X2 = _rows(X)
+    if X2.shape[0] == 0:
+        return torch.empty_like(X)
     meta, perm, inv = tl.moe_route(ids.reshape(-1).contiguous(), num_experts)
     Xs = tl.moe_gather(X2, perm, topk)
     up = tl.moe_gemm_int4(meta, Xs, Bu, Su, num_experts)

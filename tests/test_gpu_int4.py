@@ -369,6 +369,19 @@ def test_custom_operators(cuda, tl):
         torch.library.opcheck(op, args, test_utils=("test_schema", "test_faketensor"))
 
 
+def test_custom_operators_without_tokens(cuda, tl):
+    import ternocl_b200.torch_ops  # noqa: F401
+    g, E, topk, H, I = gen(2), 4, 2, 256, 128
+    X = torch.empty(0, H, dtype=torch.float16, device="cuda")
+    ids, RW = torch.ops.ternocl.moe_topk(torch.empty(0, E, device="cuda"), topk, dtype=torch.float16)
+    assert ids.shape == RW.shape == (0, topk)
+    up, down = weights(g, E, H, I, dtype=torch.float16), weights(g, E, I, H, dtype=torch.float16)
+    for op in (torch.ops.ternocl.moe_prefill_int4, torch.ops.ternocl.moe_decode_int4):
+        O = op(X, ids, RW, *up, *up, *down, E, topk)
+        assert O.shape == X.shape and O.dtype == X.dtype
+    assert torch.ops.ternocl.int4_linear(X, up[0][0], up[1][0]).shape == (0, I)
+
+
 # ------------------------------------------------------------- every kernel and schedule of the linear layer
 @pytest.mark.parametrize("bf16", [0, 1])
 @pytest.mark.parametrize("M,K,N", [
