@@ -348,7 +348,8 @@ int ternocl_moe_decode_down_sum(const int32_t *ids, const void *H, const void *R
  *   weight(k, n) = code(k, n) * S[k/128, n],   code in -8..7
  *   B : uint32 [K/8, N], code of row 8kp+j at bits 4j..4j+3 (two's complement)
  *   S : DT [K/128, N]
- * The other tensors, the epilogues and the N % 16 / K % 128 rules are ternocl_int2_upcvt's.
+ * The other tensors, the epilogues and the N % 16 / K % 128 rules are ternocl_int2_upcvt's;
+ * N <= 2^30.
  * Codes and activations are multiplied exactly and each 128-row group's fp32 sum is scaled
  * by S: no dequantised weight is rounded, at any M.  A row of A with an Inf or a NaN gives
  * values that are not finite or not meaningful in that row of C only.
@@ -356,9 +357,9 @@ int ternocl_moe_decode_down_sum(const int32_t *ids, const void *H, const void *R
  * Linear layer:  C[m,n] = DT(epi( sum_k A[m,k] * code(B[k,n]) * S[k/128, n] )).
  * algo: GEMV (decode, in blocks of 8 rows), GEMM (from 9 rows on: tcgen05, or for up to 24 rows
  * and many columns warp-level MMAs), or AUTO (the GEMV up to M = 8).  With M <= 2 the GEMV takes
- * the activations as fixed-point numbers, exact to 2^-23 of the largest of a range of K (and a
- * row with an Inf or a NaN gives NaN).  No workspace: a K
- * split stays within one thread-block cluster.  M <= 524280; C and Other 16-byte aligned. */
+ * the activations of a row as fixed-point numbers, off by at most 2^-23 of the largest of a
+ * range of K (2^-121, if that is more), and a row with an Inf or a NaN gives NaN.  No workspace:
+ * a K split stays within one thread-block cluster.  M <= 524280; C and Other 16-byte aligned. */
 int ternocl_int4_upcvt(const void *A, const uint32_t *B, const void *S, void *C, const void *Other,
                        const void *Bias, int M, int N, int K, int dtype, int postop, int out_f32, int algo,
                        void *stream);
@@ -373,7 +374,9 @@ int ternocl_moe_gemm_int4(const int32_t *meta, const void *A_all, const uint32_t
 
 /* MoE decode with 4-bit experts, as ternocl_moe_decode_gate_up and _down_sum: every routed
  * (token, expert) pair in one launch; B* [E, K/8, N], S* [E, K/128, N].  An expert id outside
- * [0, E) contributes zero and sets bit 1 of ternocl_device_error.
+ * [0, E) contributes zero, whatever its rows hold, and sets bit 1 of ternocl_device_error.
+ * Activations are taken as ternocl_int4_upcvt's at M <= 2 (down_sum: a token's valid rows of H
+ * side by side are one row).
  *   gate_up:   H[g, n] = DT(silu(X[g/topk] . gate_e[:, n]) * (X[g/topk] . up_e[:, n]))
  *   down_sum:  O[t, n] = DT(sum_j RW[g] * (H[g] . down_e[:, n])),  g = t*topk + j, e = ids[g] */
 int ternocl_moe_decode_gate_up_int4(const int32_t *ids, const void *X, const uint32_t *Bg, const void *Sg,
@@ -399,7 +402,7 @@ int ternocl_moe_decode_down_sum_int4(const int32_t *ids, const void *H, const vo
  * after the others.  A logit of +inf counts as the largest finite fp32.  Where the sum is 0 the
  * weights are 0.  So ids always holds topk distinct experts of [0, E).
  * logits [T, E] and RW [T, topk] in their own types (fp16, bf16 or fp32).  E <= 1024,
- * topk <= 32 and <= topk_group * E / n_group, n_group <= 32 dividing E. */
+ * T <= 2^30, topk <= 32 and <= topk_group * E / n_group, n_group <= 32 dividing E. */
 typedef enum { TERNOCL_SCORE_SOFTMAX = 0, TERNOCL_SCORE_SIGMOID = 1 } ternocl_score;
 int ternocl_moe_topk(const void *logits, const float *bias, int32_t *ids, void *RW, int T, int E, int topk,
                      int scoring, int n_group, int topk_group, int group_top, int renormalize, float scale,

@@ -464,6 +464,8 @@ def int4_pack(codes):
     """codes [K, N] in -8..7 -> host int4 weights (numpy uint32 [K/8, N])."""
     import numpy as np
     codes = np.asarray(codes)
+    if codes.dtype.kind not in "iu":
+        raise TypeError("codes must be integers, got %s" % codes.dtype)
     if codes.size and (codes.min() < -8 or codes.max() > 7):
         raise ValueError("codes must lie in -8..7")
     codes = np.ascontiguousarray(codes, np.int8)

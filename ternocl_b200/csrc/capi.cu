@@ -61,6 +61,7 @@ static size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 constexpr size_t kGemvSmemBudget = 100 * 1024;
 constexpr int kMaxClusterSK = 8;  // portable thread-block cluster size
 constexpr int kMaxGridYZ = 65535 * 8;  // rows whose 8-row blocks a grid's z extent holds
+constexpr int kMaxIndex = 1 << 30;  // columns or tokens that stay in 32 bits when rounded up to whole CTAs
 
 // Split-K plan of a decode GEMV whose CTAs cover `cols` columns x `rows` activation
 // rows: enough CTAs to give every SM `per_sm` of them, each CTA keeping >= 1 group
@@ -774,7 +775,7 @@ int ternocl_int4_upcvt(const void *A, const uint32_t *B, const void *S, void *C,
     int st = check_gemm_common(A, B, S, C, Other, Bias, M, N, K, dtype, postop, out_f32);
     if (st != TERNOCL_OK) return st;
     if (algo < TERNOCL_ALGO_AUTO || algo > TERNOCL_ALGO_GEMM) return TERNOCL_ERR_ARG;
-    if (M > kMaxGridYZ) return TERNOCL_ERR_SHAPE;
+    if (M > kMaxGridYZ || N > kMaxIndex) return TERNOCL_ERR_SHAPE;
     if (!aligned(C, 16) || (Other && !aligned(Other, 16))) return TERNOCL_ERR_ARG;  // 16-byte stores and loads
     if (M == 0) return TERNOCL_OK;
     GemvArgs a;
@@ -800,7 +801,7 @@ int ternocl_moe_gemm_int4(const int32_t *meta, const void *A_all, const uint32_t
     if (!meta || num_experts < 1 || num_experts > 1024) return TERNOCL_ERR_ARG;
     if (!aligned(C_all, 16) || (Other_all && !aligned(Other_all, 16))) return TERNOCL_ERR_ARG;
     // the weights' rows are one tensor map's (32-bit coordinates), the row tiles a grid's
-    if ((long long)num_experts * (K / 8) > 0x7fffffffLL || G > (1 << 20)) return TERNOCL_ERR_SHAPE;
+    if ((long long)num_experts * (K / 8) > 0x7fffffffLL || G > (1 << 20) || N > kMaxIndex) return TERNOCL_ERR_SHAPE;
     if (G == 0) return TERNOCL_OK;
     GemvArgs a;
     a.A = A_all; a.B = B_all; a.S = S_all; a.C = C_all; a.Other = Other_all;
@@ -814,7 +815,7 @@ int ternocl_moe_decode_gate_up_int4(const int32_t *ids, const void *X, const uin
                                     int num_experts, int dtype, void *stream) {
     int st = check_moe_decode(dtype, G, N, K, topk, num_experts);
     if (st != TERNOCL_OK) return st;
-    if (G % topk || (long long)G * ((N + 31) / 32) > 0x7fffffffLL) return TERNOCL_ERR_SHAPE;
+    if (N > kMaxIndex || G % topk || (long long)G * ((N + 31) / 32) > 0x7fffffffLL) return TERNOCL_ERR_SHAPE;
     if (G == 0) return TERNOCL_OK;
     if (!ids || !X || !Bg || !Sg || !Bu || !Su || !H) return TERNOCL_ERR_ARG;
     if (!aligned(X, 16) || !aligned(Bg, 16) || !aligned(Bu, 16) || !aligned(Sg, 16) || !aligned(Su, 16) ||
@@ -829,7 +830,7 @@ int ternocl_moe_decode_down_sum_int4(const int32_t *ids, const void *H, const vo
                                      int dtype, void *stream) {
     int st = check_moe_decode(dtype, T, N, K, topk, num_experts);
     if (st != TERNOCL_OK) return st;
-    if ((long long)T * ((N + 31) / 32) > 0x7fffffffLL || (long long)topk * (K / kGS) > 0x7fffffffLL ||
+    if (N > kMaxIndex || (long long)T * ((N + 31) / 32) > 0x7fffffffLL || (long long)topk * (K / kGS) > 0x7fffffffLL ||
         (long long)T * topk > 0x7fffffffLL)
         return TERNOCL_ERR_SHAPE;
     if (T == 0) return TERNOCL_OK;
@@ -850,7 +851,7 @@ int ternocl_moe_topk(const void *logits, const float *bias, int32_t *ids, void *
     if (!dt_ok(logits_dtype) || !dt_ok(rw_dtype)) return TERNOCL_ERR_ARG;
     if (scoring != TERNOCL_SCORE_SOFTMAX && scoring != TERNOCL_SCORE_SIGMOID) return TERNOCL_ERR_ARG;
     if (renormalize != 0 && renormalize != 1) return TERNOCL_ERR_ARG;
-    if (T < 0 || E < 1 || E > 1024 || topk < 1 || topk > 32) return TERNOCL_ERR_SHAPE;
+    if (T < 0 || T > kMaxIndex || E < 1 || E > 1024 || topk < 1 || topk > 32) return TERNOCL_ERR_SHAPE;
     if (n_group < 1 || n_group > 32 || E % n_group || topk_group < 1 || topk_group > n_group) return TERNOCL_ERR_SHAPE;
     if (group_top < 1 || group_top > 2 || group_top > E / n_group) return TERNOCL_ERR_SHAPE;
     if (topk > topk_group * (E / n_group)) return TERNOCL_ERR_SHAPE;

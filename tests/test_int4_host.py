@@ -29,6 +29,23 @@ def test_pack_round_trip_and_refusals():
     assert L.ternocl_int4_pack(None, 8, 2, out.ctypes.data) == 2
 
 
+def test_pack_refuses_codes_that_are_not_integers():
+    for codes in (np.full((128, 16), 1.5), np.zeros((128, 16), bool), torch.zeros(128, 16)):
+        with pytest.raises(TypeError):
+            tl.int4_pack(codes)
+
+
+def test_sizes_that_would_leave_32_bits_are_refused():
+    """Refused on the host, before any pointer is read."""
+    L, p = tl.lib(), ctypes.c_void_p(64)
+    N, T = 2 ** 31 - 16, 2 ** 31 - 1
+    assert L.ternocl_int4_upcvt(p, p, p, p, None, None, 1, N, 128, 0, 0, 0, 0, None) == 1
+    assert L.ternocl_moe_gemm_int4(p, p, p, p, p, None, 1, N, 128, 1, 0, 0, 0, None) == 1
+    assert L.ternocl_moe_decode_gate_up_int4(p, p, p, p, p, p, p, 1, N, 128, 1, 1, 0, None) == 1
+    assert L.ternocl_moe_decode_down_sum_int4(p, p, p, p, p, p, 1, N, 128, 1, 1, 0, None) == 1
+    assert L.ternocl_moe_topk(p, None, p, p, T, 1, 1, 0, 1, 1, 1, 0, 1.0, 2, 2, None) == 1
+
+
 def test_c_abi_refusals():
     L = tl.lib()
     p, q = ctypes.c_void_p(64), ctypes.c_void_p(66)  # never dereferenced
