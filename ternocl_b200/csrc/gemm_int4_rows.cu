@@ -5,8 +5,8 @@
 // Between the GEMV, whose CTAs would read the activations once per 32 columns, and the tcgen05
 // GEMM, whose decoded 16-bit operand crosses shared memory twice (48 KB of traffic per 4 KB of
 // words, 375 cycles a step whatever the rows): here a word decodes into registers as in
-// gemv_int4_core.cuh and is used for R blocks of 8 rows at once.  A CTA owns 256 columns x 8R
-// rows and a K range (split over a thread-block cluster); warp w owns 32 of the columns, streams
+// gemv_int4_core.cuh and is used for R blocks of 8 rows at once.  A CTA owns 256 columns of
+// all rows (8R at most) and a K range (split over a thread-block cluster); warp w owns 32 of the columns, streams
 // their words into registers one group ahead, and all warps share the activations of a group,
 // staged in the words' pair order in one of two buffers in shared memory.  The sums leave through
 // shared memory, so that stores and the other CTAs' shares (distributed shared memory, in split
@@ -30,7 +30,7 @@ constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kTileCols = kWarps * 32;
 constexpr int kActRow = kGS * 2 + 64;   // bytes of a staged row: 64 mod 128, 16-byte reads conflict-free
 
-struct RParams {
+struct RParams {  // M <= 8R
     const uint16_t *A;
     const uint32_t *B;
     const uint16_t *S;
@@ -53,8 +53,8 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_int4_rows_kernel(const RPara
     extern __shared__ __align__(128) char smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, t = lane & 3;
-    const int G = p.K / kGS, SK = gridDim.z, sk = blockIdx.z;
-    const int m0 = blockIdx.y * 8 * R, rows = min(8 * R, p.M - m0);
+    const int G = p.K / kGS, SK = gridDim.y, sk = blockIdx.y;
+    const int rows = min(8 * R, p.M);  // (M; the bound, told to the compiler, is worth 2 us at M = 24)
     const int g0 = (int)((long long)G * sk / SK), ng = (int)((long long)G * (sk + 1) / SK) - g0;
     const int n0 = blockIdx.x * kTileCols, ns = n0 + warp * 32;
 
@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_int4_rows_kernel(const RPara
             const int x = u * kThreads + tid, r = x >> 4;
             next[u] = make_uint4(0u, 0u, 0u, 0u);
             if (r < rows)
-                next[u] = __ldg(reinterpret_cast<const uint4 *>(p.A + (size_t)(m0 + r) * p.K + (size_t)grp * kGS) + (x & 15));
+                next[u] = __ldg(reinterpret_cast<const uint4 *>(p.A + (size_t)r * p.K + (size_t)grp * kGS) + (x & 15));
         }
     };
     auto stage = [&](int buf) {
@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_int4_rows_kernel(const RPara
             v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
             v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
         }
-        const size_t at = (size_t)(m0 + r) * p.N + n;
+        const size_t at = (size_t)r * p.N + n;
         uint4 o = make_uint4(0u, 0u, 0u, 0u);
         if constexpr (POSTOP == 1 || POSTOP == 2) o = *reinterpret_cast<const uint4 *>(p.Other + at);
         const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
@@ -204,12 +204,12 @@ template <int R>
 cudaError_t launch(const GemvArgs &a, int sms) {
     const RParams p{(const uint16_t *)a.A, a.B, (const uint16_t *)a.S, a.C, (const uint16_t *)a.Other, a.Bias,
                     a.M, a.N, a.K};
-    const int G = a.K / kGS, cols = (a.N + kTileCols - 1) / kTileCols, tiles = (a.M + 8 * R - 1) / (8 * R);
+    const int G = a.K / kGS, cols = (a.N + kTileCols - 1) / kTileCols;
     // K split: the rounds of two CTAs per SM it takes, per group, and ~2 groups' time for a CTA's ends
     int sk = 1;
     long long best = 1LL << 60;
     for (int s = 1; s <= 8 && s <= G; ++s) {
-        const long long rounds = ((long long)cols * tiles * s + 2 * sms - 1) / (2 * sms);
+        const long long rounds = ((long long)cols * s + 2 * sms - 1) / (2 * sms);
         const long long cost = rounds * ((G + s - 1) / s + 2);
         if (cost < best) {
             best = cost;
@@ -221,8 +221,8 @@ cudaError_t launch(const GemvArgs &a, int sms) {
         auto kern = gemm_int4_rows_kernel<R, DT, decltype(po)::value, decltype(of)::value>;
         const cudaError_t e = ensure_smem(kern, Smem<R>::total);
         if (e != cudaSuccess) return e;
-        return launch_kernel_cluster(kern, dim3(cols, tiles, sk), dim3(kThreads), (size_t)Smem<R>::total, a.stream,
-                                     dim3(1, 1, sk), p);
+        return launch_kernel_cluster(kern, dim3(cols, sk), dim3(kThreads), (size_t)Smem<R>::total, a.stream,
+                                     dim3(1, sk, 1), p);
     });
 }
 
