@@ -38,7 +38,7 @@
 // MMA issuer waits once per step.  Measured on B200 (bf16, CUDA graph): 14336x4096 M=2047 with
 // a residual 175-190 us = 1260-1380 TFLOP/s (floor 140 us at the burst peak), 4096x4096 M=2048
 // 57 us, 4096x4096 M=64 11.9 us; grouped 32768 rows x 768 x 2048 over 128 experts with SwiGLU
-// 175 us (floor 60), 536 rows 46 us (16.4).
+// 175 us (floor 60).
 // Every mbarrier wait is bounded (tc::mbar_wait); on a timeout the roles stop, the producers
 // wait (bounded) for their copies in flight, and TMEM is freed.
 #include <cuda.h>
@@ -842,6 +842,10 @@ cudaError_t int4_gemm_launch(const GemvArgs &a, int sms, const int *meta, int E)
     // at M = 16 23.5 against 31.6 us here, at M = 24 28.5 against 33.0; 4096x6144 at M = 16 10.9 against 12.5;
     // 14336x4096 at M = 16 23.4 against 17.2.
     if (!meta && a.M <= kInt4RowsMaxM && (long long)((a.N + 255) / 256) * 8 >= sms) return int4_rows_launch(a, sms);
+    // Grouped, up to 8 rows per expert on average by gemv_int4.cu (K 2048, 768 columns, 128 experts: 1 row
+    // each 18.9 against 35.1 us here, 4 28.8 / 46.3, 8 40.8 / 52.1, 12.5 55.7 / 53.1; K 4096, 14336 columns, 8
+    // experts: 6 rows 62 / 87, 12 rows 108 / 93).
+    if (meta && per <= kInt4GemvMaxM) return int4_gemv_grouped_launch(a, meta, E);
     int MT = per <= 32 ? 32 : per <= 64 ? 64 : per <= 128 ? 128 : 256;
     const long long strips = (a.N + gemm4::BN - 1) / gemm4::BN;
     if (MT == 256 && !meta) {

@@ -7,6 +7,8 @@
 // gemv::finish, in a fixed order.
 //
 // M <= 2: the same on the integer form, for ranges of up to kStage groups per warp.
+// Grouped by expert, with 8 rows per expert or fewer on average: the M >= 3 form on the rows of one
+// expert in blocks of 8.
 //
 // Bound by HBM, with issue close behind (the 16-bit form needs 314 instructions per group and
 // warp, the integer one ~110).  Weights go straight to registers: no ring in shared memory
@@ -17,9 +19,10 @@
 // next strip's words on their way (134 against 130 us).
 // Measured on B200 (bf16, CUDA graph, us; floor = words and scales at 6.45 TB/s): 4096x4096 M=1 4.45
 // (1.3), M=8 5.65; 4096x28672 M=1 17.1 (9.4), M=8 20.2; 5376x21504 M=1 15.6 (9.3), M=8 17.3;
-// 14336x4096 M=1 10.9 (4.7); 5120x248320 M=1 126 (102), M=8 156.  ncu, 5120x124160 M=1
-// (profiles/int4_gemv_gemm.md): DRAM reads = words + scales, issue 54 % busy, 256 instructions
-// per group and warp with a CTA's ends counted in.
+// 14336x4096 M=1 10.9 (4.7); 5120x248320 M=1 126 (102), M=8 156.  ncu, 5120x124160 M=1:
+// DRAM reads = words + scales, issue 54 % busy, 256 instructions per group and warp with a CTA's
+// ends counted in.  Grouped, 536 rows x 2048 x 768 over 128 experts 28.8 us (floor 16.4; 46 us on
+// the tcgen05 kernel, whose tiles would hold 4 rows), 128 rows 18.9.
 #include <cuda_runtime.h>
 
 #include "gemv_common.cuh"
@@ -101,6 +104,81 @@ __global__ void __launch_bounds__(W * 32, 24 / W) gemv_int4_digit_kernel(const g
     gemv::finish<Int4Cols, W, DT, POSTOP, OUT_F32>(p, smem, v, n0 + 4 * g < p.N);
 }
 
+// ---- the grouped product for a few rows per expert ----------------------------------------
+// CTA (x, y): 32 columns of expert y's first 8 rows; y >= E: of the (y - E)-th of the further blocks of
+// 8 rows, counted over the experts, most of which do not exist.
+struct GroupedParams {
+    const int *meta;
+    const uint16_t *A;
+    const uint32_t *B;
+    const uint16_t *S;
+    void *C;
+    const uint16_t *Other;
+    int M, N, K, E;
+};
+
+template <int W, class DT, int POSTOP, bool OUT_F32>
+__global__ void __launch_bounds__(W * 32, 24 / W) gemv_int4_grouped_kernel(const GroupedParams p) {
+    __shared__ __align__(16) float red[W][32][8];  // partial sums
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int g = lane >> 2, t = lane & 3;
+    const int n0 = blockIdx.x * 32, G = p.K / kGS;
+    pdl_wait();  // meta comes from the routing kernel
+    int e = blockIdx.y, block = 0;
+    auto first = [&](int x) { return min(max(p.meta[x], 0), p.M); };
+    auto count = [&](int x) { return x < p.E ? max(first(x + 1) - first(x), 0) : 0; };
+    if (e >= p.E) {
+        int want = e - p.E, e0 = 0;
+        for (;; e0 += 32) {
+            if (e0 >= p.E) return;  // (every warp finds the same)
+            const int own = max(count(e0 + lane) - 1, 0) / 8;
+            int incl = own;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += y;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, incl > want);
+            if (past) {
+                const int l = __ffs(past) - 1;
+                e = e0 + l;
+                block = 1 + want - __shfl_sync(0xffffffffu, incl - own, l);
+                break;
+            }
+            want -= __shfl_sync(0xffffffffu, incl, 31);
+        }
+    }
+    const int rows = min(count(e) - 8 * block, 8), row0 = first(e) + 8 * block;
+    if (rows <= 0) return;
+    const int g0 = G * warp / W, g1 = G * (warp + 1) / W;
+    float acc[2][4] = {};
+    if (g0 < g1) {
+        int4::WordStream st;
+        st.width(p.N);
+        st.seek(p.B, p.S, p.N, e * G + g0, n0, lane);
+        st.load();
+        int4::multiply<DT>(st, p.A + (size_t)(row0 + (g < rows ? g : 0)) * p.K + (size_t)g0 * kGS + 8 * t, g < rows,
+                           g1 - g0, 1.0f, acc);
+    }
+    pdl_launch_dependents();
+    *reinterpret_cast<float4 *>(&red[warp][lane][0]) = make_float4(acc[0][0], acc[0][2], acc[1][0], acc[1][2]);
+    *reinterpret_cast<float4 *>(&red[warp][lane][4]) = make_float4(acc[0][1], acc[0][3], acc[1][1], acc[1][3]);
+    __syncthreads();
+    // columns c, c + 1 of row m: lane (c / 4, m / 2)'s
+    for (int m = tid >> 4; m < rows; m += 2 * W) {
+        const int c = 2 * (tid & 15);
+        if (n0 + c >= p.N) break;
+        float v0 = 0.0f, v1 = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float2 x = *reinterpret_cast<const float2 *>(&red[w][c / 4 * 4 + m / 2][(m & 1) * 4 + (c & 3)]);
+            v0 += x.x;
+            v1 += x.y;
+        }
+        epi_store2<DT, POSTOP, OUT_F32, OUT_F32>(p.C, p.Other, nullptr, p.N, row0 + m, n0 + c, v0, v1);
+    }
+}
+
 template <int W, int ROWS, class DT, int POSTOP, bool OUT_F32>
 cudaError_t launch_digit(const GemvArgs &a, int most) {
     const gemv::Params p = gemv::gemv_params_impl(a);
@@ -134,6 +212,21 @@ cudaError_t int4_gemv_launch(const GemvArgs &a) {
         constexpr bool F32 = decltype(of)::value;
         if (a.warps >= 8) return launch_w<8, DT, PO, F32>(a);
         return launch_w<4, DT, PO, F32>(a);
+    });
+}
+
+// 4 warps split K, or 2 where that left a warp fewer than 4 groups: 536 rows over 128 experts, K 2048,
+// 768 columns 28.8 us with 4 and 28.1 with 2, and 128 rows 18.9 and 21.5; K 768, 2048 columns 40.7 and 30.9.
+cudaError_t int4_gemv_grouped_launch(const GemvArgs &a, const int *meta, int E) {
+    const GroupedParams p{meta, (const uint16_t *)a.A, a.B, (const uint16_t *)a.S, a.C, (const uint16_t *)a.Other,
+                          a.M, a.N, a.K, E};
+    return dispatch_epilogue<GemvArgs>(a, [&](auto dt, auto po, auto of) {
+        using DT = typename decltype(dt)::type;
+        constexpr int PO = decltype(po)::value;
+        constexpr bool F32 = decltype(of)::value;
+        const dim3 grid((a.N + 31) / 32, E + a.M / 8);
+        if (a.K / kGS >= 16) return launch_kernel(gemv_int4_grouped_kernel<4, DT, PO, F32>, grid, dim3(128), 0, a.stream, p);
+        return launch_kernel(gemv_int4_grouped_kernel<2, DT, PO, F32>, grid, dim3(64), 0, a.stream, p);
     });
 }
 

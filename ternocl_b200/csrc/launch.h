@@ -221,6 +221,7 @@ cudaError_t moe_topk_launch(const MoeTopkArgs &a);
 // int4 GEMV (gemv_int4.cu), GEMM (gemm_int4.cu; grouped with meta) and MoE decode GEMVs
 // (moe_decode_int4.cu)
 cudaError_t int4_gemv_launch(const GemvArgs &a);
+cudaError_t int4_gemv_grouped_launch(const GemvArgs &a, const int *meta, int E);
 cudaError_t int4_gemm_launch(const GemvArgs &a, int sms, const int *meta = nullptr, int E = 0);
 // the int4 product for up to kInt4RowsMaxM rows (gemm_int4_rows.cu)
 constexpr int kInt4RowsMaxM = 24;
@@ -233,7 +234,7 @@ cudaError_t moe_decode_down_sum_int4_launch(const int *ids, const void *H, const
                                             const void *S, void *O, int T, int N, int K, int topk, int E, int dtype,
                                             int sms, cudaStream_t st);
 cudaError_t read_device_error_moe_decode_int4(unsigned *out, int reset);
-// largest M that TERNOCL_ALGO_AUTO gives the int4 GEMV
+// largest M (grouped: average rows of an expert) that TERNOCL_ALGO_AUTO gives the int4 GEMV
 constexpr int kInt4GemvMaxM = 8;
 // M from which TERNOCL_ALGO_AUTO picks the GEMM (int2_fp16_upcvt/main.cpp:160)
 constexpr int kGemmMinM = 64;

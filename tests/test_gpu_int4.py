@@ -283,6 +283,35 @@ def test_grouped_gemm_segments_and_rows_behind_them(cuda, tl, counts):
     assert tl.device_error() == 0
 
 
+@pytest.mark.parametrize("K,N", [(384, 144), (2176, 48)])
+@pytest.mark.parametrize("counts", [[0] * 70 + [200] + [0, 1, 7, 8, 9, 16, 17] * 4 + [0], [8, 9, 0, 7], [1] * 40,
+                                    [0] * 31 + [60] + [33] + [0] * 31, [0, 0, 0, 24]])
+def test_grouped_gemm_few_rows_per_expert(cuda, tl, counts, K, N):
+    """Up to 8 rows per expert on average, unevenly: blocks of 8 rows beyond an expert's first, experts
+    beyond a warp's lanes, rows before the first segment and behind the last untouched."""
+    g = gen(sum(counts) + K)
+    E, before, behind = len(counts), 3, 5
+    G = before + sum(counts) + behind
+    A = activations(g, G, K, torch.float16)
+    A[:before] = A[G - behind:] = float("nan")
+    B, S = weights(g, E, K, N, dtype=torch.float16)
+    S = (S / K ** 0.5).half()
+    other = torch.randn(G, N, generator=g, device="cuda").half()
+    rows = before + np.concatenate([[0], np.cumsum(counts)])
+    tiles = np.concatenate([[0], np.cumsum([(c + 127) // 128 for c in counts])])
+    meta = torch.tensor(np.concatenate([rows, tiles]), dtype=torch.int32, device="cuda")
+    C = torch.full((G, N), -7.0, device="cuda", dtype=torch.float16)
+    tl.moe_gemm_int4(meta, A, B, S, E, postop=2, other=other, out=C)
+    for e in range(E):
+        lo, hi = int(rows[e]), int(rows[e + 1])
+        if hi > lo:
+            v, d = product64(A[lo:hi], matrix64(B[e], S[e]), False)
+            want, bound = epilogue64(v, d, 2, other[lo:hi], None, True)
+            check(C[lo:hi], want, bound, "expert %d" % e)
+    assert bool((C[:before] == -7.0).all()) and bool((C[G - behind:] == -7.0).all())
+    assert tl.device_error() == 0
+
+
 def test_expert_weights_beyond_32_bit_offsets(cuda, tl):
     """The last expert's words start behind 4 GiB."""
     E, K, N = 1024, 4096, 2048
