@@ -7,19 +7,20 @@
 // gemv::finish, in a fixed order.
 //
 // M <= 2: the same on the integer form, for ranges of up to kStage groups per warp.
+//
 // Grouped by expert, with 8 rows per expert or fewer on average: the M >= 3 form on the rows of one
 // expert in blocks of 8.
 //
 // Bound by HBM, with issue close behind (the 16-bit form needs 314 instructions per group and
 // warp, the integer one ~110).  Weights go straight to registers: no ring in shared memory
-// leaves ~24 resident warps per SM with 2 KB each in flight, and a warp nothing to wait for
+// leaves 24 to 28 resident warps per SM with 2 KB each in flight, and a warp nothing to wait for
 // before its first words (on the cp.async ring of gemv_common.cuh 5120x248320 at M = 2 took
 // 223 us, 2.9 TB/s).  Reading further ahead (2 to 4 groups at 80 to 128 registers) measured
 // the same or slower, and so did CTAs that walk several strips with the planes kept and the
 // next strip's words on their way (134 against 130 us).
 // Measured on B200 (bf16, CUDA graph, us; floor = words and scales at 6.45 TB/s): 4096x4096 M=1 4.45
-// (1.3), M=8 5.65; 4096x28672 M=1 17.1 (9.4), M=8 20.2; 5376x21504 M=1 15.6 (9.3), M=8 17.3;
-// 14336x4096 M=1 10.9 (4.7); 5120x248320 M=1 126 (102), M=8 156.  ncu, 5120x124160 M=1:
+// (1.3), M=8 5.65; 4096x28672 M=1 14.7 (9.4), M=8 20.2; 5376x21504 M=1 15.3 (9.3), M=8 17.3;
+// 14336x4096 M=1 10.9 (4.7); 5120x248320 M=1 122 (102), M=2 147, M=8 156.  ncu, 5120x124160 M=1:
 // DRAM reads = words + scales, issue 54 % busy, 256 instructions per group and warp with a CTA's
 // ends counted in.  Grouped, 536 rows x 2048 x 768 over 128 experts 28.8 us (floor 16.4; 46 us on
 // the tcgen05 kernel, whose tiles would hold 4 rows), 128 rows 18.9.
@@ -65,8 +66,9 @@ __global__ void __launch_bounds__(W * 32, 24 / W) gemv_int4_kernel(const gemv::P
     gemv::finish<Int4Cols, W, DT, POSTOP, OUT_F32>(p, smem, v, n0 + 4 * g < p.N);
 }
 
+// (one row: 7 CTAs of 4 warps on an SM, at 72 registers)
 template <int W, int ROWS, class DT, int POSTOP, bool OUT_F32>
-__global__ void __launch_bounds__(W * 32, 24 / W) gemv_int4_digit_kernel(const gemv::Params p, int pbytes) {
+__global__ void __launch_bounds__(W * 32, (ROWS == 1 ? 28 : 24) / W) gemv_int4_digit_kernel(const gemv::Params p, int pbytes) {
     extern __shared__ __align__(128) char smem[];  // [W][32][8] partial sums, then the warps' planes
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2;
