@@ -204,25 +204,22 @@ static GemvPlan gemv_i8_plan(int M, int N, int K, bool allow_ws) {
     return p;
 }
 
-// int4 GEMV (gemv_int4.cu): 32 columns x 8 rows per CTA, 24 warps resident per SM (28 for M = 1 with
-// 4 warps per CTA); split-K within a cluster.  Measured from CUDA graphs (bf16, us, 8 warps / 4
-// warps per CTA):
+// int4 GEMV (gemv_int4.cu): 32 columns x 8 rows per CTA; an SM holds 3 CTAs of 8 warps or 7 of 4;
+// split-K within a cluster.  Measured from CUDA graphs (bf16, us, 8 warps / 4 warps per CTA):
 //  - K is split while the strips leave SMs without a CTA and every warp keeps 4 groups:
 //    14336x4096 M=1 one CTA per strip 14.7, two 10.9; 4096x4096 4.4 and 5.0;
-//  - M = 1: 4 warps where their rounds of 7 CTAs per SM, counted in strips, are below 1.2 times
-//    the rounds of 3 of 8 warps: 4096x28672 (6.05 strips per SM) 17.3 / 14.7, 5376x21504 17.1 /
-//    15.3, 5120x65536 39.5 / 33.4, 5120x248320 136 / 122, but 5120x34816 (7.35) 23.3 / 25.0;
-//  - else 4 warps where their 6 CTAs per SM hold all strips and the 3 of 8 warps do not (5376x21504
-//    M=8 19.5 / 17.2; 4096x28672 has 8 strips too many: 20.4 / 21.0), and for many rounds of strips
-//    (5120x248320 M=8 164 / 155), but for M = 2, whose digit planes then take the SM's whole shared
-//    memory (150 / 168).
+//  - 4 warps where their rounds of 7 CTAs per SM, counted in strips, are below 1.2 times the
+//    rounds of 3 of 8 warps: 4096x28672 (6.05 strips per SM) M=1 17.3 / 14.7, M=8 19.5 / 17.3;
+//    5376x21504 M=1 17.1 / 15.3, M=8 19.0 / 16.6; 5120x65536 39.5 / 33.4 and 42.7 / 39.9;
+//    5120x248320 136 / 122 and 160 / 148; but 5120x34816 (7.35) M=1 23.3 / 25.0;
+//  - M = 2: 4 warps where 6 CTAs per SM hold all strips and 3 of 8 warps do not, else 8: the digit
+//    planes of 4-warp CTAs take the SM's whole shared memory (5120x248320 150 / 168).
 static GemvPlan gemv_i4_plan(int M, int N, int K) {
     const int G = K / kGS, sms = sm_count();
     const long long tiles = (long long)((N + 31) / 32) * ((M + 7) / 8);
     auto rounds = [&](int ctas) { return ctas * ((tiles + ctas * sms - 1) / (ctas * sms)); };
     GemvPlan p;
-    if (M == 1) p.warps = 5 * rounds(7) < 6 * rounds(3) ? 4 : 8;
-    else p.warps = (tiles > 3LL * sms && tiles <= 6LL * sms) || (tiles > 24LL * sms && M != 2) ? 4 : 8;
+    p.warps = (M == 2 ? tiles > 3LL * sms && tiles <= 6LL * sms : 5 * rounds(7) < 6 * rounds(3)) ? 4 : 8;
     if (const int forced = options().gemv_warps) p.warps = forced >= 8 ? 8 : 4;
     while (p.SK < kMaxClusterSK && 8 * p.SK * p.warps <= G && tiles * p.SK * 2 <= 3LL * sms) p.SK *= 2;
     if (const int forced = options().gemv_split) p.SK = std::min({forced, G, kMaxClusterSK});

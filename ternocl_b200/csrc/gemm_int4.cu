@@ -843,8 +843,8 @@ cudaError_t int4_gemm_launch(const GemvArgs &a, int sms, const int *meta, int E)
     // 14336x4096 at M = 16 23.4 against 17.2.
     if (!meta && a.M <= kInt4RowsMaxM && (long long)((a.N + 255) / 256) * 8 >= sms) return int4_rows_launch(a, sms);
     // Grouped, up to 8 rows per expert on average by gemv_int4.cu (K 2048, 768 columns, 128 experts: 1 row
-    // each 18.9 against 35.1 us here, 4 28.8 / 46.3, 8 40.8 / 52.1, 12.5 55.7 / 53.1; K 4096, 14336 columns, 8
-    // experts: 6 rows 62 / 87, 12 rows 108 / 93).
+    // each 18.0 against 35.1 us here, 4 28.5 / 46.3, 8 39.3 / 52.1, 12.5 55.7 / 53.1; K 4096, 14336 columns, 8
+    // experts: 6 rows 60 / 87, 12 rows 108 / 93).
     if (meta && per <= kInt4GemvMaxM) return int4_gemv_grouped_launch(a, meta, E);
     int MT = per <= 32 ? 32 : per <= 64 ? 64 : per <= 128 ? 128 : 256;
     const long long strips = (a.N + gemm4::BN - 1) / gemm4::BN;

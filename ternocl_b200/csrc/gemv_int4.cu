@@ -19,11 +19,11 @@
 // the same or slower, and so did CTAs that walk several strips with the planes kept and the
 // next strip's words on their way (134 against 130 us).
 // Measured on B200 (bf16, CUDA graph, us; floor = words and scales at 6.45 TB/s): 4096x4096 M=1 4.45
-// (1.3), M=8 5.65; 4096x28672 M=1 14.7 (9.4), M=8 20.2; 5376x21504 M=1 15.3 (9.3), M=8 17.3;
-// 14336x4096 M=1 10.9 (4.7); 5120x248320 M=1 122 (102), M=2 147, M=8 156.  ncu, 5120x124160 M=1:
+// (1.3), M=8 5.65; 4096x28672 M=1 14.7 (9.4), M=8 17.3; 5376x21504 M=1 15.3 (9.3), M=8 16.6;
+// 14336x4096 M=1 10.9 (4.7); 5120x248320 M=1 122 (102), M=2 147, M=8 148.  ncu, 5120x124160 M=1:
 // DRAM reads = words + scales, issue 54 % busy, 256 instructions per group and warp with a CTA's
-// ends counted in.  Grouped, 536 rows x 2048 x 768 over 128 experts 28.8 us (floor 16.4; 46 us on
-// the tcgen05 kernel, whose tiles would hold 4 rows), 128 rows 18.9.
+// ends counted in.  Grouped, 536 rows x 2048 x 768 over 128 experts 28.5 us (floor 16.4; 46 us on
+// the tcgen05 kernel, whose tiles would hold 4 rows), 128 rows 18.0.
 #include <cuda_runtime.h>
 
 #include "gemv_common.cuh"
@@ -40,8 +40,11 @@ struct Int4Cols {
     __device__ static int thread_col(int g, int i) { return 4 * g + i; }
 };
 
+// warps on an SM, at 72 registers: 7 CTAs of 4 warps, or 3 of 8
+constexpr int kResident = 28;
+
 template <int W, class DT, int POSTOP, bool OUT_F32>
-__global__ void __launch_bounds__(W * 32, 24 / W) gemv_int4_kernel(const gemv::Params p) {
+__global__ void __launch_bounds__(W * 32, kResident / W) gemv_int4_kernel(const gemv::Params p) {
     extern __shared__ __align__(128) char smem[];  // [W][32][8] partial sums
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
@@ -66,9 +69,10 @@ __global__ void __launch_bounds__(W * 32, 24 / W) gemv_int4_kernel(const gemv::P
     gemv::finish<Int4Cols, W, DT, POSTOP, OUT_F32>(p, smem, v, n0 + 4 * g < p.N);
 }
 
-// (one row: 7 CTAs of 4 warps on an SM, at 72 registers)
+// (two rows' planes leave no room for more CTAs)
 template <int W, int ROWS, class DT, int POSTOP, bool OUT_F32>
-__global__ void __launch_bounds__(W * 32, (ROWS == 1 ? 28 : 24) / W) gemv_int4_digit_kernel(const gemv::Params p, int pbytes) {
+__global__ void __launch_bounds__(W * 32, (ROWS == 1 ? kResident : 24) / W)
+    gemv_int4_digit_kernel(const gemv::Params p, int pbytes) {
     extern __shared__ __align__(128) char smem[];  // [W][32][8] partial sums, then the warps' planes
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2;
@@ -120,7 +124,7 @@ struct GroupedParams {
 };
 
 template <int W, class DT, int POSTOP, bool OUT_F32>
-__global__ void __launch_bounds__(W * 32, 24 / W) gemv_int4_grouped_kernel(const GroupedParams p) {
+__global__ void __launch_bounds__(W * 32, kResident / W) gemv_int4_grouped_kernel(const GroupedParams p) {
     __shared__ __align__(16) float red[W][32][8];  // partial sums
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, t = lane & 3;
@@ -218,7 +222,8 @@ cudaError_t int4_gemv_launch(const GemvArgs &a) {
 }
 
 // 4 warps split K, or 2 where that left a warp fewer than 4 groups: 536 rows over 128 experts, K 2048,
-// 768 columns 28.8 us with 4 and 28.1 with 2, and 128 rows 18.9 and 21.5; K 768, 2048 columns 40.7 and 30.9.
+// 768 columns 28.8 us with 4 and 28.1 with 2, and 128 rows 18.9 and 21.5; K 768, 2048 columns 40.7 and 30.9
+// (24 resident warps).
 cudaError_t int4_gemv_grouped_launch(const GemvArgs &a, const int *meta, int E) {
     const GroupedParams p{meta, (const uint16_t *)a.A, a.B, (const uint16_t *)a.S, a.C, (const uint16_t *)a.Other,
                           a.M, a.N, a.K, E};
