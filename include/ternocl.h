@@ -284,7 +284,9 @@ int ternocl_bitcos_upcvt_hadamard(const void *A, const int8_t *signs, int use_si
  *
  * Route, replaces int2_moe_route (int2_moe_prefill.cl:30-31): from ids[G] (expert of
  * row g = t*topk + j) build meta[2E+2] = [E+1 row offsets | E+1 row-tile offsets],
- * perm[G] (sorted row p -> g, ascending g inside an expert) and inv[G] (g -> p).
+ * perm[G] (sorted row p -> g, ascending g inside an expert) and inv[G] (g -> p).  A row whose
+ * id lies outside [0, num_experts) is left out: inv[g] = -1, and perm[p] = -1 from
+ * p = meta[num_experts] on; gather makes zero rows of those p, combine adds nothing for that g.
  * rows_per_tile must equal ternocl_moe_rows_per_tile() for ternocl_moe_gemm. */
 int ternocl_moe_rows_per_tile(void);
 int ternocl_moe_route(const int32_t *ids, int32_t *meta, int32_t *perm, int32_t *inv, int G,

@@ -247,7 +247,8 @@ def moe_rows_per_tile():
 
 
 def moe_route(ids, num_experts, stream=None):
-    """ids int32 [G] (expert of routed row g = t*topk + j) -> (meta [2E+2], perm [G], inv [G])."""
+    """ids int32 [G] (expert of routed row g = t*topk + j) -> (meta [2E+2], perm [G], inv [G]).
+    A row whose id lies outside [0, E) is left out: inv is -1 there, and perm from p = meta[E] on."""
     torch = _torch()
     _check_cuda(ids)
     G = ids.numel()
@@ -260,7 +261,7 @@ def moe_route(ids, num_experts, stream=None):
 
 
 def moe_gather(X, perm, topk, out=None, stream=None):
-    """Xs[p] = X[perm[p] / topk]."""
+    """Xs[p] = X[perm[p] / topk], zeros where perm[p] < 0."""
     torch = _torch()
     _check_cuda(X, perm, out)
     G = perm.numel()
@@ -310,7 +311,7 @@ def moe_gemm_i8(meta, Aq, SA, B_all, SB_all, num_experts, postop=0, out_f32=Fals
 
 
 def moe_combine(Y, inv, RW, T, topk, out=None, stream=None):
-    """O[t] = sum_j RW[t*topk+j] * Y[inv[t*topk+j]]; Y fp32 [G, N], RW [G] fp16/bf16."""
+    """O[t] = sum_j RW[t*topk+j] * Y[inv[t*topk+j]] over the j with inv >= 0; Y fp32 [G, N], RW [G] fp16/bf16."""
     torch = _torch()
     _check_cuda(Y, inv, RW, out)
     N = Y.shape[1]

@@ -2,9 +2,9 @@
 //
 //   route    (int2_moe_route, :29-61)   rows per expert, meta = [E+1 row offsets |
 //            E+1 row-tile offsets], perm (sorted row -> routed row g) and inv (g -> row)
-//   gather   (int2_moe_gather, :63-70)  Xs[p] = X[perm[p] / topk]
+//   gather   (int2_moe_gather, :63-70)  Xs[p] = X[perm[p] / topk], zeros where perm[p] < 0
 //   combine  (int2_moe_combine, :143-156) O[t, n] = DT(sum_j RW[g] * Y[inv[g], n]),
-//            g = t*topk + j, j in increasing order, fp32 sum
+//            g = t*topk + j, j in increasing order, fp32 sum; without the j where inv[g] < 0
 //   gather_q (int2_moe_gather_q, int2_moe_prefill_int8.cl:73-84) the int8 variant: int8
 //            rows and their per-group activation scales into expert order
 //
@@ -16,8 +16,9 @@
 // the reference's single work-group): counts with shared-memory atomics, then a row's
 // position is its expert's offset + the count of the same expert in lower warps (a
 // 32-step scan per expert) + its rank among the lanes of its warp with the same expert
-// (__match_any_sync); beyond that one CTA per 1024 rows (moe_route_mc_kernel).  Expert
-// ids outside [0, E) are skipped and flagged in the device error word (bit 1).
+// (__match_any_sync); beyond that one CTA per 1024 rows (moe_route_mc_kernel).  A row whose
+// expert id lies outside [0, E) is left out and flagged in the device error word (bit 1): its
+// inv is -1, and the places of perm that no row takes, from meta[E] on, hold -1.
 #include <cuda_runtime.h>
 
 #include "common.cuh"
@@ -35,6 +36,7 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(const int *__r
     int *cnt = sm;          // [E] rows per expert, then the running offset
     int *tot = sm + E;      // [E] this round's rows per expert
     int *wc = sm + 2 * E;   // [32][E] per-warp counts -> exclusive prefix over warps
+    __shared__ int taken;   // rows of all experts
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_wait();
     for (int e = tid; e < E; e += kRouteThreads) cnt[e] = 0;
@@ -60,8 +62,10 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(const int *__r
         }
         meta[E] = r;
         meta[2 * E + 1] = t;
+        taken = r;
     }
     __syncthreads();
+    for (int p = taken + tid; p < G; p += kRouteThreads) perm[p] = -1;
     for (int base = 0; base < G; base += kRouteThreads) {
         const int g = base + tid;
         int e = g < G ? ids[g] : -1;
@@ -85,6 +89,8 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(const int *__r
             const int p = cnt[e] + wc[warp * E + e] + rank;
             perm[p] = g;
             inv[g] = p;
+        } else if (g < G) {
+            inv[g] = -1;
         }
         __syncthreads();
         for (int x = tid; x < E; x += kRouteThreads) cnt[x] += tot[x];
@@ -105,6 +111,7 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_mc_kernel(const int *
     int *tot = sm;          // [E] rows per expert (all G)
     int *base = sm + E;     // [E] first row of this chunk's rows of expert e
     int *wc = sm + 2 * E;   // [32][E]
+    __shared__ int taken;   // rows of all experts
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int c0 = blockIdx.x * kRouteThreads;
     pdl_wait();
@@ -142,9 +149,11 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_mc_kernel(const int *
             meta[E] = r;
             meta[2 * E + 1] = t;
         }
+        taken = r;
     }
     __syncthreads();
     const int g = c0 + tid;
+    if (g >= taken && g < G) perm[g] = -1;  // (place g of perm)
     int e = g < G ? ids[g] : -1;
     if (e >= E) e = -1;
     const unsigned peers = __match_any_sync(0xffffffffu, e);
@@ -164,17 +173,24 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_mc_kernel(const int *
         const int pos = base[e] + wc[warp * E + e] + rank;
         perm[pos] = g;
         inv[g] = pos;
+    } else if (g < G) {
+        inv[g] = -1;
     }
     pdl_launch_dependents();
 }
 
-// one CTA row: Xs[p] = X[perm[p] / topk], 16-byte copies
+// one CTA row: Xs[p] = X[perm[p] / topk] (zeros where perm[p] < 0), 16-byte copies
 __global__ void __launch_bounds__(256) moe_gather_kernel(const uint4 *__restrict__ X, const int *__restrict__ perm,
                                                         uint4 *__restrict__ Xs, int G, int K8, int topk) {
     pdl_wait();
     for (int p = blockIdx.x; p < G; p += gridDim.x) {
-        const uint4 *src = X + (size_t)(perm[p] / topk) * K8;
+        const int g = perm[p];
         uint4 *dst = Xs + (size_t)p * K8;
+        if (g < 0) {
+            for (int k = threadIdx.x; k < K8; k += blockDim.x) dst[k] = make_uint4(0u, 0u, 0u, 0u);
+            continue;
+        }
+        const uint4 *src = X + (size_t)(g / topk) * K8;
         for (int k = threadIdx.x; k < K8; k += blockDim.x) dst[k] = src[k];
     }
     pdl_launch_dependents();
@@ -182,7 +198,7 @@ __global__ void __launch_bounds__(256) moe_gather_kernel(const uint4 *__restrict
 
 // int8 rows and their activation scales into expert order (int2_moe_gather_q,
 // int2_moe/int2_moe_prefill_int8.cl:73-84): Xsq[p] = Xq[t], SA[g, p] = SAt[g, t] with
-// t = perm[p] / topk and the scale pitches LDSA(T), LDSA(G)
+// t = perm[p] / topk and the scale pitches LDSA(T), LDSA(G); zeros where perm[p] < 0
 __global__ void __launch_bounds__(256) moe_gather_q_kernel(const uint4 *__restrict__ Xq,
                                                           const uint16_t *__restrict__ SAt,
                                                           const int *__restrict__ perm, uint4 *__restrict__ Xsq,
@@ -191,9 +207,14 @@ __global__ void __launch_bounds__(256) moe_gather_q_kernel(const uint4 *__restri
     const int K16 = K / 16, ngroups = K / kGS;
     const size_t ldt = (size_t)((T + 31) & ~31), ldg = (size_t)((G + 31) & ~31);
     for (int p = blockIdx.x; p < G; p += gridDim.x) {
-        const int t = perm[p] / topk;
-        const uint4 *src = Xq + (size_t)t * K16;
+        const int row = perm[p], t = row / topk;
         uint4 *dst = Xsq + (size_t)p * K16;
+        if (row < 0) {
+            for (int k = threadIdx.x; k < K16; k += blockDim.x) dst[k] = make_uint4(0u, 0u, 0u, 0u);
+            for (int g = threadIdx.x; g < ngroups; g += blockDim.x) SA[g * ldg + p] = 0;
+            continue;
+        }
+        const uint4 *src = Xq + (size_t)t * K16;
         for (int k = threadIdx.x; k < K16; k += blockDim.x) dst[k] = src[k];
         for (int g = threadIdx.x; g < ngroups; g += blockDim.x) SA[g * ldg + p] = SAt[g * ldt + t];
     }
@@ -212,9 +233,10 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(const float *__restric
         const int t = (int)(idx / n4), c = (int)(idx % n4) * 4;
         float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
         for (int j = 0; j < topk; ++j) {
-            const int g = t * topk + j;
+            const int g = t * topk + j, p = inv[g];
+            if (p < 0) continue;  // left out: its row of Y is nobody's
             const float w = DT::tof(RW[g]);
-            const float4 y = *reinterpret_cast<const float4 *>(Y + (size_t)inv[g] * N + c);
+            const float4 y = *reinterpret_cast<const float4 *>(Y + (size_t)p * N + c);
             s0 += w * y.x;
             s1 += w * y.y;
             s2 += w * y.z;
