@@ -202,12 +202,27 @@ def _(logits, topk, bias=None, scoring="softmax", n_group=1, topk_group=1, group
     return logits.new_empty(shape, dtype=torch.int32), logits.new_empty(shape, dtype=dtype or logits.dtype)
 
 
+def _check_routed(X2, ids, RW, topk):
+    """ids and RW hold topk entries for each row of X2, of the types that the kernels read."""
+    rows = X2.shape[0] * topk
+    if topk < 1 or ids.numel() != rows or RW.numel() != rows:
+        raise ValueError("ids and RW must hold topk = %d entries for each of the %d tokens, got %d and %d"
+                         % (topk, X2.shape[0], ids.numel(), RW.numel()))
+    if ids.dtype != torch.int32 or RW.dtype != X2.dtype:
+        raise TypeError("ids must be int32 and RW %s as X, got %s and %s" % (X2.dtype, ids.dtype, RW.dtype))
+    if ids.device != X2.device or RW.device != X2.device:
+        raise ValueError("ids and RW must be on %s as X, got %s and %s" % (X2.device, ids.device, RW.device))
+
+
 @torch.library.custom_op(_NS + "::moe_prefill_int4", mutates_args=())
 def moe_prefill_int4(X: torch.Tensor, ids: torch.Tensor, RW: torch.Tensor, Bg: torch.Tensor, Sg: torch.Tensor,
                      Bu: torch.Tensor, Su: torch.Tensor, Bd: torch.Tensor, Sd: torch.Tensor, num_experts: int,
                      topk: int) -> torch.Tensor:
     """moe_prefill with 4-bit experts: B* int32 [E, K/8, N], S* [E, K/128, N]."""
     X2 = _rows(X)
+    _check_routed(X2, ids, RW, topk)
+    if Bd.shape[-1] != X2.shape[1]:
+        raise ValueError("Bd must lead back to the %d columns of X, got %d" % (X2.shape[1], Bd.shape[-1]))
     if X2.shape[0] == 0:
         return torch.empty_like(X)
     meta, perm, inv = tl.moe_route(ids.reshape(-1).contiguous(), num_experts)

@@ -126,6 +126,29 @@ def test_custom_operator_shapes():
         assert op(X, ids, W, W, W, W, W, W, W, 16, 8).shape == X.shape
 
 
+def test_prefill_layer_refuses_routing_that_does_not_fit():
+    """Refused before anything is launched: ids and weights that are too few, too many or of another type would be
+    read as other memory or as other numbers."""
+    T, E, topk, H, I = 6, 4, 2, 256, 128
+    X = torch.zeros(T, H).half()
+    ids, RW = torch.zeros(T, topk, dtype=torch.int32), torch.zeros(T, topk).half()
+    up = torch.zeros(E, H // 8, I, dtype=torch.int32), torch.zeros(E, H // 128, I).half()
+    down = torch.zeros(E, I // 8, H, dtype=torch.int32), torch.zeros(E, I // 128, H).half()
+    wide = torch.zeros(E, I // 8, 2 * H, dtype=torch.int32), torch.zeros(E, I // 128, 2 * H).half()
+    op = torch.ops.ternocl.moe_prefill_int4
+    for kind, what, args in (
+            (ValueError, "entries", (ids[:-1], RW)), (ValueError, "entries", (ids.repeat(2, 1), RW)),
+            (ValueError, "entries", (ids, RW[:, :1])), (ValueError, "entries", (ids, RW.repeat(1, 2))),
+            (TypeError, "int32", (ids.long(), RW)), (TypeError, "int32", (ids, RW.float())),
+            (TypeError, "int32", (ids, RW.bfloat16()))):
+        with pytest.raises(kind, match=what):
+            op(X, *args, *up, *up, *down, E, topk)
+    with pytest.raises(ValueError, match="entries"):
+        op(X, ids[:, :0], RW[:, :0], *up, *up, *down, E, 0)
+    with pytest.raises(ValueError, match="lead back"):
+        op(X, ids, RW, *up, *up, *wide, E, topk)
+
+
 def test_reference_choice_by_hand():
     """The 64-bit definition on a case small enough to do by hand."""
     ids, w = topk64([[0.0, 1.0, 1.0, -1.0]], 2, scoring="sigmoid", renormalize=False)
