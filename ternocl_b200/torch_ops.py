@@ -225,12 +225,13 @@ def moe_prefill_int4(X: torch.Tensor, ids: torch.Tensor, RW: torch.Tensor, Bg: t
         raise ValueError("Bd must lead back to the %d columns of X, got %d" % (X2.shape[1], Bd.shape[-1]))
     if X2.shape[0] == 0:
         return torch.empty_like(X)
-    meta, perm, inv = tl.moe_route(ids.reshape(-1).contiguous(), num_experts)
-    Xs = tl.moe_gather(X2, perm, topk)
-    up = tl.moe_gemm_int4(meta, Xs, Bu, Su, num_experts)
-    H = tl.moe_gemm_int4(meta, Xs, Bg, Sg, num_experts, postop=1, other=up)
-    Y = tl.moe_gemm_int4(meta, H, Bd, Sd, num_experts, out_f32=True)
-    return tl.moe_combine(Y, inv, RW.reshape(-1).contiguous(), X2.shape[0], topk).reshape(X.shape)
+    with torch.cuda.device(X2.device):  # (route, gather and combine launch on the current device)
+        meta, perm, inv = tl.moe_route(ids.reshape(-1).contiguous(), num_experts)
+        Xs = tl.moe_gather(X2, perm, topk)
+        up = tl.moe_gemm_int4(meta, Xs, Bu, Su, num_experts)
+        H = tl.moe_gemm_int4(meta, Xs, Bg, Sg, num_experts, postop=1, other=up)
+        Y = tl.moe_gemm_int4(meta, H, Bd, Sd, num_experts, out_f32=True)
+        return tl.moe_combine(Y, inv, RW.reshape(-1).contiguous(), X2.shape[0], topk).reshape(X.shape)
 
 
 @moe_prefill_int4.register_fake

@@ -149,6 +149,42 @@ def test_prefill_layer_refuses_routing_that_does_not_fit():
         op(X, ids, RW, *up, *up, *wide, E, topk)
 
 
+def test_prefill_layer_runs_on_the_device_of_its_inputs(monkeypatch):
+    """Every launch of the layer, also when another device is current."""
+    current, entered = [None], []
+
+    class Device:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            entered.append(self.device)
+            current[0] = self.device
+
+        def __exit__(self, *_):
+            current[0] = None
+
+    T, E, topk, H, I = 6, 4, 2, 256, 128
+    X = torch.zeros(T, H).half()
+
+    def stub(out):
+        def f(*args, **kw):
+            assert current[0] == X.device
+            return out
+        return f
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(tl, "moe_route", stub((None, None, None)))
+    for name in ("moe_gather", "moe_gemm_int4"):
+        monkeypatch.setattr(tl, name, stub(X))
+    monkeypatch.setattr(tl, "moe_combine", stub(X.clone()))
+    up = torch.zeros(E, H // 8, I, dtype=torch.int32), torch.zeros(E, H // 128, I).half()
+    down = torch.zeros(E, I // 8, H, dtype=torch.int32), torch.zeros(E, I // 128, H).half()
+    ids, RW = torch.zeros(T, topk, dtype=torch.int32), torch.zeros(T, topk).half()
+    torch.ops.ternocl.moe_prefill_int4(X, ids, RW, *up, *up, *down, E, topk)
+    assert entered == [X.device]
+
+
 def test_reference_choice_by_hand():
     """The 64-bit definition on a case small enough to do by hand."""
     ids, w = topk64([[0.0, 1.0, 1.0, -1.0]], 2, scoring="sigmoid", renormalize=False)
