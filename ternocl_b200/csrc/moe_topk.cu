@@ -345,14 +345,21 @@ __global__ void __launch_bounds__(kWarps * 32) moe_topk_kernel(const TopkParams 
         read_token<L, IPL>(p, t, l, open, mx);
         int id = 0;
         float w = 0.0f;
-        // fp32: |s - its 64-bit value| <= 2^-21 s + 2^-24 (expf 2 ulp of a rounded argument, the sum and the
-        // quotient; x exp(-x) < 1/2), and c is off by 2^-24 |c| more
+        // What fp32 can be off by, in units of u = 2^-24.  A sigmoid: expf 2 ulp (4 u), a sum and a quotient,
+        // 6 u s.  A softmax: expf 4 u, its argument 0.4 u (|x - mx| is off by itself times u, and
+        // d exp(-d) < 0.37); of the sum, expf 4 u, the arguments 4.5 u (the mean of |x - mx| weighted by
+        // the terms, of 1024 experts), 10 additions (pairwise in a lane, then over lanes); the quotient and the
+        // product: 24.5 u s + 0.4 u, taken as 32 u s + 0.5 u.  c is off by u |c| more.
         float inv = 1.0f;  // softmax: 1 / sum over the experts (renormalised weights alone do without)
         if (softmax && (p.bias || grouped || !p.renorm)) {
-            float sum = 0.0f;
+            float term[IPL];
 #pragma unroll
-            for (int i = 0; i < IPL; ++i) sum += (open >> i) & 1u ? expf(l[i] - mx) : 0.0f;
-            inv = 1.0f / seg_sum<L>(sum);
+            for (int i = 0; i < IPL; ++i) term[i] = (open >> i) & 1u ? expf(l[i] - mx) : 0.0f;
+#pragma unroll
+            for (int o = IPL / 2; o > 0; o >>= 1)
+#pragma unroll
+                for (int i = 0; i < o; ++i) term[i] += term[i + o];
+            inv = 1.0f / seg_sum<L>(term[0]);
         }
         auto score = [&](float x) { return softmax ? expf(x - mx) * inv : 1.0f / (1.0f + expf(-x)); };
         const bool indexed = !p.bias && p.logits_dtype != TERNOCL_FP32;
@@ -397,7 +404,7 @@ __global__ void __launch_bounds__(kWarps * 32) moe_topk_kernel(const TopkParams 
             if (lo > 1u && hi > 1u) {  // (masked groups are ordered by index)
                 const float a = __int_as_float(lo >> 31 ? lo & 0x7fffffffu : ~lo);
                 const float b = __int_as_float(hi >> 31 ? hi & 0x7fffffffu : ~hi);
-                sure = a - b > 0x1p-17f + 0x1p-20f * fmaxf(fabsf(a), fabsf(b));
+                sure = sure && a - b > 0x1p-17f + 0x1p-20f * fmaxf(fabsf(a), fabsf(b));
             }
 #pragma unroll
             for (int i = 0; i < IPL; ++i)
@@ -426,7 +433,8 @@ __global__ void __launch_bounds__(kWarps * 32) moe_topk_kernel(const TopkParams 
             if (sl < p.topk && its > 1u && next > 1u) {
                 const float a = __int_as_float(its >> 31 ? its & 0x7fffffffu : ~its);
                 const float b = __int_as_float(next >> 31 ? next & 0x7fffffffu : ~next);
-                sure = sure && a - b > 0x1p-20f * (w + ws) + 0x1p-22f + 0x1p-22f * fmaxf(fabsf(a), fabsf(b));
+                const float rel = softmax ? 0x1p-19f : 0x1p-20f;
+                sure = sure && a - b > rel * (w + ws) + 0x1p-22f + 0x1p-22f * fmaxf(fabsf(a), fabsf(b));
             }
         }
         if (p.renorm) {

@@ -156,3 +156,24 @@ def test_many_tokens(cuda, tl, E, topk, scoring, biased, groups):
         logits[-1] = 0.5
         bias = 0.1 * torch.randn(E, generator=g, device="cuda") if biased else None
         run(tl, logits, topk, bias=bias, scoring=scoring, renormalize=dtype != torch.float16, **groups)
+
+
+@pytest.mark.parametrize("T,E", [(70, 1024), (70, 512), (2050, 512), (2050, 300)])
+def test_near_ties_behind_a_sum_of_many_small_terms(cuda, tl, T, E):
+    """A softmax of one large and 31 small terms, each below half a step of the running sum in 32 bits: an expert
+    whose choice value lies within the sum of what those additions lose comes out as in 64 bits."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(E)
+    logits = torch.full((T, E), -100.0, device="cuda")
+    logits[:, 0] = 0.0
+    logits[:, 1:32] = -15.9 - 3.0 * torch.rand(T, 31, generator=g, device="cuda")
+    logits[0, 1:32] = float(np.log(2.0 ** -24))
+    logits[1, 1:32] = -16.62
+    bias = torch.full((E,), -5.0, device="cuda")
+    bias[0], bias[100] = -1.0, -1.5e-6
+    for renorm in (False, True):
+        run(tl, logits, 1, bias=bias, renormalize=renorm)
+        run(tl, logits, 3, bias=bias, renormalize=renorm)
+    bias = torch.zeros(E, device="cuda")
+    bias[40] = 1.0 - 33 * 2.0 ** -24
+    run(tl, logits, 1, bias=bias, renormalize=False)
