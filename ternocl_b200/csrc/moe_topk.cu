@@ -398,7 +398,10 @@ __global__ void __launch_bounds__(kWarps * 32) moe_topk_kernel(const TopkParams 
                 const int first = seg_first<L>(k == seg_max<L>(k));
                 if ((lane - first) / span == 0 && lane >= first) kept = true;
             }
-            // the least kept score against the best of the others
+            // the least kept score against the best of the others: two groups' scores (a softmax's sum to 1 at
+            // most, four sigmoids) are off by 34 u; their c by |b1| + |b2| <= |total| + 2 * 16 u each, with larger
+            // opposites left to 64 bits; the totals by |total| u: less than 128 u + 16 u max |total|
+            if (p.group_top == 2 && real && b1 > 0.0f && b2 < -16.0f) sure = false;
             const unsigned lo = ~seg_max<L>(kept && real ? ~gkey : 0u);
             const unsigned hi = seg_max<L>(!kept && real ? gkey : 0u);
             if (lo > 1u && hi > 1u) {  // (masked groups are ordered by index)

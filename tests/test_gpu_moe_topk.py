@@ -177,3 +177,19 @@ def test_near_ties_behind_a_sum_of_many_small_terms(cuda, tl, T, E):
     bias = torch.zeros(E, device="cuda")
     bias[40] = 1.0 - 33 * 2.0 ** -24
     run(tl, logits, 1, bias=bias, renormalize=False)
+
+
+@pytest.mark.parametrize("T", [300, 2500])
+@pytest.mark.parametrize("per", [2, 4])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_group_scores_whose_biases_cancel(cuda, tl, T, per, scoring):
+    """Groups whose two best biases are 1000 and -1000: their scores are small and of what 32 bits lose of the
+    two choice values."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(per)
+    n_group = 4
+    logits = 2e-4 * torch.randn(T, per * n_group, generator=g, device="cuda")
+    bias = torch.full((n_group, per), float("-inf"), device="cuda")
+    bias[:, 0] = 1000.0 + 0.25 * torch.arange(n_group)
+    bias[:, 1] = -bias[:, 0]
+    run(tl, logits, 2, bias=bias.reshape(-1), scoring=scoring, n_group=n_group, topk_group=1, group_top=2)
