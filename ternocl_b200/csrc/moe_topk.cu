@@ -17,7 +17,8 @@
 // bias the scores rise with the logits, and the logits themselves are compared, exactly.
 // Else the choice is first made on fp32 scores, one expert past topk, and stands if every gap
 // between neighbours exceeds what fp32 can be off by; a token that fails the test (1 in 100
-// or fewer on random logits, and exact ties) is done again in 64 bits.
+// or fewer on random logits, and exact ties) is done again in 64 bits, and so is one that
+// chooses a score below 2^-100.
 //
 // A segment of 32 or 16 lanes per token: lane l holds experts IPL l .. IPL l + IPL - 1, so that
 // a group is a few neighbouring lanes.  A value becomes an unsigned key that orders as the value
@@ -417,8 +418,12 @@ __global__ void __launch_bounds__(kWarps * 32) moe_topk_kernel(const TopkParams 
         const int steps = min(p.topk + (p.bias ? 1 : 0), L);
         if (indexed) take_indexed<L, IPL>(key, steps, id, its);
         else take<L, IPL>(key, steps, id, its);
-        if (indexed ? its >= 2048u : its > 1u)  // unmasked
+        if (indexed ? its >= 2048u : its > 1u) {  // unmasked
             w = score(fminf(logit_at(p, (size_t)t * p.E + id), FLT_MAX));
+            // scores near the end of fp32's range (a sigmoid far below 0, a softmax's far below its largest)
+            // would lose bits or vanish, and with them the weights that they are divided into
+            if (sl < p.topk && w < 0x1p-100f) sure = false;
+        }
         if (p.bias) {
             // neighbours in the order (and the first one left out; at topk = 32 the rest's best)
             unsigned next = __shfl_down_sync(kAll, its, 1);

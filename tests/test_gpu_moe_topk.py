@@ -193,3 +193,40 @@ def test_group_scores_whose_biases_cancel(cuda, tl, T, per, scoring):
     bias[:, 0] = 1000.0 + 0.25 * torch.arange(n_group)
     bias[:, 1] = -bias[:, 0]
     run(tl, logits, 2, bias=bias.reshape(-1), scoring=scoring, n_group=n_group, topk_group=1, group_top=2)
+
+
+@pytest.mark.parametrize("T", [5, 2100])
+def test_chosen_scores_at_the_end_of_32_bits(cuda, tl, T):
+    """All chosen scores so small that 32 bits hold them as 0 or with few bits: their ratios are the weights."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(7)
+    for E, groups in ((24, {}), (32, dict(n_group=8, topk_group=3, group_top=2))):
+        noise = torch.rand(T, E, generator=g, device="cuda")
+        for level in (-70.0, -88.0, -89.0, -100.0, -104.0, -150.0, -700.0):
+            for dtype in TYPES:  # sigmoids far below 0
+                logits = (level + noise).to(dtype)
+                run(tl, logits, 8, scoring="sigmoid", **groups)
+                run(tl, logits, 8, scoring="sigmoid", bias=torch.rand(E, generator=g, device="cuda"), **groups)
+        logits = torch.full((T, 8), -100.0, device="cuda")
+        assert bool((tl.moe_topk(logits, 8, scoring="sigmoid", scale=2.0)[1] == 0.25).all())
+
+
+@pytest.mark.parametrize("T", [5, 2100])
+@pytest.mark.parametrize("below", [50.0, 90.0, 110.0, 600.0])
+def test_chosen_scores_far_below_the_softmax_maximum(cuda, tl, T, below):
+    """A bias, or the choice of groups, leaves out the row's largest logit."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(8)
+    E = 16
+    # whole multiples of 1/8, so that every difference is exact in 32 bits
+    logits = -below + 0.125 * torch.randint(0, 16, (T, E), generator=g, device="cuda")
+    logits[:, 0] = 0.0
+    bias = torch.rand(E, generator=g, device="cuda")
+    bias[0] = -10.0
+    for renorm in (False, True):
+        run(tl, logits, 4, bias=bias, renormalize=renorm)
+        # group 0 has no second unmasked expert
+        alone = logits.clone()
+        alone[:, 1:4] = float("-inf")
+        run(tl, alone, 4, n_group=4, topk_group=2, group_top=2, renormalize=renorm)
+        run(tl, alone, 4, bias=bias, n_group=4, topk_group=2, group_top=2, renormalize=renorm)
