@@ -419,7 +419,14 @@ __global__ void __launch_bounds__(kWarps * 32) moe_topk_kernel(const TopkParams 
         if (indexed) take_indexed<L, IPL>(key, steps, id, its);
         else take<L, IPL>(key, steps, id, its);
         if (indexed ? its >= 2048u : its > 1u) {  // unmasked
-            w = score(fminf(logit_at(p, (size_t)t * p.E + id), FLT_MAX));
+            const float x = fminf(logit_at(p, (size_t)t * p.E + id), FLT_MAX);
+            w = score(x);
+            if (softmax) {
+                // d = x - mx is off by up to |d| u, which the weight would be off by: what the subtraction
+                // rounded away, times w (beyond 128 the token is computed in 64 bits)
+                const float d = x - mx, b = d - x;
+                if (d > -128.0f) w = fmaf(w, (x - (d - b)) - (mx + b), w);
+            }
             // scores near the end of fp32's range (a sigmoid far below 0, a softmax's far below its largest)
             // would lose bits or vanish, and with them the weights that they are divided into
             if (sl < p.topk && w < 0x1p-100f) sure = false;

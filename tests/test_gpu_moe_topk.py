@@ -230,3 +230,17 @@ def test_chosen_scores_far_below_the_softmax_maximum(cuda, tl, T, below):
         alone[:, 1:4] = float("-inf")
         run(tl, alone, 4, n_group=4, topk_group=2, group_top=2, renormalize=renorm)
         run(tl, alone, 4, bias=bias, n_group=4, topk_group=2, group_top=2, renormalize=renorm)
+
+
+@pytest.mark.parametrize("T", [5, 2100])
+@pytest.mark.parametrize("E,biased", [(64, False), (64, True), (600, False)])
+def test_weights_of_logits_far_apart(cuda, tl, T, E, biased):
+    """Logits tens below the largest one: their difference to it is rounded in 32 bits, their weight is not off by
+    that rounding."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(9)
+    logits = 65.0 * torch.rand(T, E, generator=g, device="cuda")
+    bias = torch.rand(E, generator=g, device="cuda") if biased else None
+    for renorm in (False, True):
+        run(tl, logits, 12, bias=bias, renormalize=renorm)
+        run(tl, logits - 1000.0, 12, bias=bias, renormalize=renorm)
