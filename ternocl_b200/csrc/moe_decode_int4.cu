@@ -51,7 +51,7 @@ template <int W, int MODE, class DT>
 __global__ void __launch_bounds__(W * 32, 16 / W) moe_decode_int4_kernel(const MParams p) {
     constexpr int NM = kMats<MODE>;
     extern __shared__ __align__(128) char smem[];  // the warps' planes
-    __shared__ float red[W][NM][kCols];
+    __shared__ __align__(16) float red[W][NM][kCols];  // (written 16 bytes at a time)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int z = blockIdx.x / p.strips;  // routed row (gate_up) or token (down_sum)
     const int n0 = (blockIdx.x - z * p.strips) * kCols;
