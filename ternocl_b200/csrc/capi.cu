@@ -211,15 +211,13 @@ static GemvPlan gemv_i8_plan(int M, int N, int K, bool allow_ws) {
 //  - 4 warps where their rounds of 7 CTAs per SM, counted in strips, are below 1.2 times the
 //    rounds of 3 of 8 warps: 4096x28672 (6.05 strips per SM) M=1 17.3 / 14.7, M=8 19.5 / 17.3;
 //    5376x21504 M=1 17.1 / 15.3, M=8 19.0 / 16.6; 5120x65536 39.5 / 33.4 and 42.7 / 39.9;
-//    5120x248320 136 / 122 and 160 / 148; but 5120x34816 (7.35) M=1 23.3 / 25.0;
-//  - M = 2: 4 warps where 6 CTAs per SM hold all strips and 3 of 8 warps do not, else 8: the digit
-//    planes of 4-warp CTAs take the SM's whole shared memory (5120x248320 150 / 168).
+//    5120x248320 136 / 122 and 160 / 148; but 5120x34816 (7.35) M=1 23.3 / 25.0.
 static GemvPlan gemv_i4_plan(int M, int N, int K) {
     const int G = K / kGS, sms = sm_count();
     const long long tiles = (long long)((N + 31) / 32) * ((M + 7) / 8);
     auto rounds = [&](int ctas) { return ctas * ((tiles + ctas * sms - 1) / (ctas * sms)); };
     GemvPlan p;
-    p.warps = (M == 2 ? tiles > 3LL * sms && tiles <= 6LL * sms : 5 * rounds(7) < 6 * rounds(3)) ? 4 : 8;
+    p.warps = 5 * rounds(7) < 6 * rounds(3) ? 4 : 8;
     if (const int forced = options().gemv_warps) p.warps = forced >= 8 ? 8 : 4;
     while (p.SK < kMaxClusterSK && 8 * p.SK * p.warps <= G && tiles * p.SK * 2 <= 3LL * sms) p.SK *= 2;
     if (const int forced = options().gemv_split) p.SK = std::min({forced, G, kMaxClusterSK});

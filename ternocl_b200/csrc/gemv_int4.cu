@@ -2,13 +2,15 @@
 //
 //   C[m,n] = DT(epi( sum_g S[g,n] * sum_{k in g} A[m,k] * code(B[k,n]) ))
 //
-// M >= 3: a CTA owns 32 columns, up to 8 activation rows and a K range, which its W warps (and
+// M >= 2: a CTA owns 32 columns, up to 8 activation rows and a K range, which its W warps (and
 // SK CTAs of a cluster) split by 128-row groups (gemv_int4_core.cuh); the partial sums meet in
 // gemv::finish, in a fixed order.
 //
-// M <= 2: the same on the integer form, for ranges of up to kStage groups per warp.
+// M = 1: the same on the integer form, for ranges of up to kStage groups per warp.  (With the digits
+// of two rows it was slower than the 16-bit form: 4096x28672 M=2 21.1 against 18.6 us, 4096x4096
+// 5.5 / 5.1, 14336x4096 12.8 / 11.9, 5120x34816 25.9 / 24.9, 5120x248320 148.9 / 147.7.)
 //
-// Grouped by expert, with 8 rows per expert or fewer on average: the M >= 3 form on the rows of one
+// Grouped by expert, with 8 rows per expert or fewer on average: the M >= 2 form on the rows of one
 // expert in blocks of 8.
 //
 // Bound by HBM, with issue close behind (the 16-bit form needs 314 instructions per group and
@@ -69,9 +71,8 @@ __global__ void __launch_bounds__(W * 32, kResident / W) gemv_int4_kernel(const 
     gemv::finish<Int4Cols, W, DT, POSTOP, OUT_F32>(p, smem, v, n0 + 4 * g < p.N);
 }
 
-// (two rows' planes leave no room for more CTAs)
-template <int W, int ROWS, class DT, int POSTOP, bool OUT_F32>
-__global__ void __launch_bounds__(W * 32, (ROWS == 1 ? kResident : 24) / W)
+template <int W, class DT, int POSTOP, bool OUT_F32>
+__global__ void __launch_bounds__(W * 32, kResident / W)
     gemv_int4_digit_kernel(const gemv::Params p, int pbytes) {
     extern __shared__ __align__(128) char smem[];  // [W][32][8] partial sums, then the warps' planes
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -87,26 +88,21 @@ __global__ void __launch_bounds__(W * 32, (ROWS == 1 ? kResident : 24) / W)
         st.load();
     }
     pdl_wait();  // the weights are on their way; the activations are the previous kernel's
-    int4::DigitRows<ROWS, DT> rows;
-    rows.pbytes = pbytes;
-    rows.planes = smem + W * 1024 + warp * 3 * ROWS * pbytes;
-    rows.stage(p.A + (size_t)g0 * kGS, p.K, ng, lane);
+    int4::DigitRow<DT> row;
+    row.pbytes = pbytes;
+    row.planes = smem + W * 1024 + warp * 3 * pbytes;
+    row.stage(p.A + (size_t)g0 * kGS, ng, lane);
     float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
     for (int i = 0; i < ng; ++i) {
         const uint4 w[4] = {st.w[0], st.w[1], st.w[2], st.w[3]};
         const uint2 s4 = st.s;
         if (i + 1 < ng) st.load();
-        rows.group(w, s4, 1.0f, i, lane, acc);
+        row.group(w, s4, 1.0f, i, lane, acc);
     }
     pdl_launch_dependents();
     float total[4] = {0.f, 0.f, 0.f, 0.f};
-    if (ng > 0) rows.finish(acc, lane, total);  // (ng is the same for the whole warp)
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        v[j] = total[j];                                                                     // row 2t
-        v[4 + j] = ROWS == 2 ? __shfl_down_sync(0xffffffffu, total[j], 2) : 0.0f;  // row 2t + 1: from lane t = 2
-    }
+    if (ng > 0) row.finish(acc, total);  // (ng is the same for the whole warp)
+    float v[8] = {total[0], total[1], total[2], total[3], 0.f, 0.f, 0.f, 0.f};  // row 2t (of t = 0)
     gemv::finish<Int4Cols, W, DT, POSTOP, OUT_F32>(p, smem, v, n0 + 4 * g < p.N);
 }
 
@@ -185,12 +181,12 @@ __global__ void __launch_bounds__(W * 32, kResident / W) gemv_int4_grouped_kerne
     }
 }
 
-template <int W, int ROWS, class DT, int POSTOP, bool OUT_F32>
+template <int W, class DT, int POSTOP, bool OUT_F32>
 cudaError_t launch_digit(const GemvArgs &a, int most) {
     const gemv::Params p = gemv::gemv_params_impl(a);
-    auto kern = gemv_int4_digit_kernel<W, ROWS, DT, POSTOP, OUT_F32>;
+    auto kern = gemv_int4_digit_kernel<W, DT, POSTOP, OUT_F32>;
     const int pbytes = int4::plane_bytes(most);
-    const size_t smem = (size_t)W * (1024 + 3 * ROWS * pbytes);
+    const size_t smem = (size_t)W * (1024 + 3 * pbytes);
     const cudaError_t e = ensure_smem(kern, smem);
     if (e != cudaSuccess) return e;
     return launch_kernel_cluster(kern, dim3((a.N + 31) / 32, a.SK), dim3(W * 32), smem, a.stream,
@@ -200,8 +196,7 @@ cudaError_t launch_digit(const GemvArgs &a, int most) {
 template <int W, class DT, int POSTOP, bool OUT_F32>
 cudaError_t launch_w(const GemvArgs &a) {
     const int G = a.K / kGS, most = ((G + a.SK - 1) / a.SK + W - 1) / W;  // groups of any warp
-    if (a.M == 1 && most <= int4::kStage) return launch_digit<W, 1, DT, POSTOP, OUT_F32>(a, most);
-    if (a.M == 2 && most <= int4::kStage) return launch_digit<W, 2, DT, POSTOP, OUT_F32>(a, most);
+    if (a.M == 1 && most <= int4::kStage) return launch_digit<W, DT, POSTOP, OUT_F32>(a, most);
     const gemv::Params p = gemv::gemv_params_impl(a);
     auto kern = gemv_int4_kernel<W, DT, POSTOP, OUT_F32>;
     const dim3 grid((a.N + 31) / 32, a.SK, (a.M + 7) / 8);

@@ -9,16 +9,16 @@
 // the same K rows, from L1.  Products of codes and DT activations are exact in the MMA's fp32
 // sums; a group's sum is scaled by S in fp32.
 //
-// For one or two rows there is an integer form with a third of the instructions: a word is two
+// For one row there is an integer form with a third of the instructions: a word is two
 // A registers of mma.sync m16n8k32 s8 x s8 (its even and odd rows as 16 * code, three
 // operations for eight weights), against digit planes of the activations.  With 2^e such that
 // |A| * 2^e < 2^22 (digit_common.cuh), i = round(A * 2^e) is split into three balanced base-256
 // digits, i = d0 + 256 d1 + 65536 d2 with d in [-128, 127]: adding 0x808080 makes them the bytes
-// of a positive number, and flipping each top bit makes those bytes signed.  Of the MMA's
-// eight n-columns 3m .. 3m+2 are the planes of row m; a group's dots (|sum 16 code d| <=
+// of a positive number, and flipping each top bit makes those bytes signed.  The planes are
+// the first three of the MMA's eight n-columns; a group's dots (|sum 16 code d| <=
 // 128 * 128 * 128 = 2^21) are exact and read as floats from the accumulator's start pattern.
 // Elements more than 2^11 below the largest of the row's range lose bits beyond fp16's, at
-// most 2^-23 of that largest.  (5120x248320 at M = 1: 130 us against 150 us in 16 bits.)
+// most 2^-22 of that largest.  (5120x248320 at M = 1: 130 us against 150 us in 16 bits.)
 #pragma once
 #include "common.cuh"
 #include "digit_common.cuh"
@@ -160,42 +160,38 @@ __device__ __forceinline__ void word_digits(const uint4 v, int e, uint2 (&out)[3
     for (int d = 0; d < 3; ++d) out[d] = make_uint2(r[0][d], r[1][d]);
 }
 
-// One or two activation rows of up to kStage groups as digit planes in the warp's shared memory.
-template <int ROWS, class DT>
-struct DigitRows {
-    static_assert(ROWS <= 2, "one MMA holds the planes of two rows");
+// An activation row of up to kStage groups as digit planes in the warp's shared memory.
+template <class DT>
+struct DigitRow {
     char *planes;
-    int pbytes;      // of a plane
-    float rs[ROWS];  // what an integer of row m's planes counts
+    int pbytes;  // of a plane
+    float rs;    // what an integer of the planes counts
 
     // `use(group)`: false has that group's activations taken as zeros
     template <class Use>
-    __device__ __forceinline__ void stage(const uint16_t *a0, size_t a_stride, int ng, int lane, Use use) {
+    __device__ __forceinline__ void stage(const uint16_t *a0, int ng, int lane, Use use) {
         __syncwarp();  // the planes' last readers are through
-#pragma unroll
-        for (int m = 0; m < ROWS; ++m) {
-            const uint4 *a = reinterpret_cast<const uint4 *>(a0 + m * a_stride);
-            uint32_t mx = 0;
+        const uint4 *a = reinterpret_cast<const uint4 *>(a0);
+        uint32_t mx = 0;
 #pragma unroll 1
-            for (int u = lane; u < 16 * ng; u += 32)
-                if (use(u >> 4)) mx = max(mx, absmax_bits(__ldg(a + u)));
-            mx = __reduce_max_sync(0xffffffffu, mx);
-            const int e = digit::exponent_for<DT>(mx);
-            rs[m] = inverse_scale<DT>(mx, e);
+        for (int u = lane; u < 16 * ng; u += 32)
+            if (use(u >> 4)) mx = max(mx, absmax_bits(__ldg(a + u)));
+        mx = __reduce_max_sync(0xffffffffu, mx);
+        const int e = digit::exponent_for<DT>(mx);
+        rs = inverse_scale<DT>(mx, e);
 #pragma unroll 1
-            for (int u = lane; u < 16 * ng; u += 32) {  // word row u
-                uint2 d[3];
-                word_digits<DT>(use(u >> 4) ? __ldg(a + u) : make_uint4(0u, 0u, 0u, 0u), e, d);
-                char *dst = planes + 3 * m * pbytes + (u / 16) * 128 + (u & 3) * 32 + ((u >> 2) & 3) * 8;
+        for (int u = lane; u < 16 * ng; u += 32) {  // word row u
+            uint2 d[3];
+            word_digits<DT>(use(u >> 4) ? __ldg(a + u) : make_uint4(0u, 0u, 0u, 0u), e, d);
+            char *dst = planes + (u / 16) * 128 + (u & 3) * 32 + ((u >> 2) & 3) * 8;
 #pragma unroll
-                for (int k = 0; k < 3; ++k) *reinterpret_cast<uint2 *>(dst + k * pbytes) = d[k];
-            }
+            for (int k = 0; k < 3; ++k) *reinterpret_cast<uint2 *>(dst + k * pbytes) = d[k];
         }
         __syncwarp();
     }
 
-    __device__ __forceinline__ void stage(const uint16_t *a0, size_t a_stride, int ng, int lane) {
-        stage(a0, a_stride, ng, lane, [](int) { return true; });
+    __device__ __forceinline__ void stage(const uint16_t *a0, int ng, int lane) {
+        stage(a0, ng, lane, [](int) { return true; });
     }
 
     // acc += (staged group i) x w, scaled by s4 * factor: acc[b][c] is column 4g + 2b + (c >> 1),
@@ -203,8 +199,8 @@ struct DigitRows {
     __device__ __forceinline__ void group(const uint4 (&w)[4], const uint2 s4, float factor, int i, int lane,
                                           float (&acc)[2][4]) const {
         const int g = lane >> 2, t = lane & 3;
-        const char *b0 = planes + (g < 3 * ROWS ? g : 0) * pbytes + t * 32 + i * 128;
-        const uint32_t mask = g < 3 * ROWS ? 0xffffffffu : 0u;
+        const char *b0 = planes + (g < 3 ? g : 0) * pbytes + t * 32 + i * 128;
+        const uint32_t mask = g < 3 ? 0xffffffffu : 0u;
         int32_t d[2][4];
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -230,20 +226,15 @@ struct DigitRows {
                 acc[b][c] = fmaf(__int_as_float(d[b][c]) - digit::kMagic, s[2 * b + (c >> 1)], acc[b][c]);
     }
 
-    // total[m][j] += row m of acc at column 4g + j, in the lanes with t = 0 (row 0) and t = 2 (row 1)
-    __device__ __forceinline__ void finish(const float (&acc)[2][4], int lane, float (&total)[4]) const {
-        const int t = lane & 3;
+    // total[j] += acc's planes at column 4g + j, in the lanes with t = 0
+    __device__ __forceinline__ void finish(const float (&acc)[2][4], float (&total)[4]) const {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                // planes 2t, 2t+1 here and 2t+2, 2t+3 in the next lane: row 0 is planes 0, 1, 2 (from
-                // lane t = 0), row 1 is planes 3, 4, 5 (from t = 2: plane 3 is lane t = 1's second)
-                const float lo = acc[b][2 * c], hi = acc[b][2 * c + 1];
-                const float next = __shfl_down_sync(0xffffffffu, lo, 1);
-                const float prev = __shfl_up_sync(0xffffffffu, hi, 1);
-                const float r = t == 0 ? (lo + 256.0f * hi) + 65536.0f * next : (prev + 256.0f * lo) + 65536.0f * hi;
-                total[2 * b + c] = fmaf(r, t == 0 ? rs[0] : rs[ROWS - 1], total[2 * b + c]);
+                const float next = __shfl_down_sync(0xffffffffu, acc[b][2 * c], 1);  // plane 2
+                const float r = (acc[b][2 * c] + 256.0f * acc[b][2 * c + 1]) + 65536.0f * next;
+                total[2 * b + c] = fmaf(r, rs, total[2 * b + c]);
             }
     }
 };

@@ -58,9 +58,9 @@ __global__ void __launch_bounds__(W * 32, 16 / W) moe_decode_int4_kernel(const M
     const int G = p.K / kGS;
     const int all = MODE == kGateUp ? G : p.topk * G;
     const int g0 = (int)((long long)all * warp / W), ng = (int)((long long)all * (warp + 1) / W) - g0;
-    int4::DigitRows<1, DT> rows;
-    rows.pbytes = int4::plane_bytes((all + W - 1) / W);
-    rows.planes = smem + warp * 3 * rows.pbytes;
+    int4::DigitRow<DT> row;
+    row.pbytes = int4::plane_bytes((all + W - 1) / W);
+    row.planes = smem + warp * 3 * row.pbytes;
 
     pdl_wait();  // ids and activations come from the kernels before
 
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) moe_decode_int4_kernel(const M
             };
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) unit(k, k);
-            rows.stage(a0 + (size_t)c0 * kGS, 0, nc, lane);
+            row.stage(a0 + (size_t)c0 * kGS, nc, lane);
             float acc[2][2][4];
 #pragma unroll
             for (int m = 0; m < 2; ++m)
@@ -112,11 +112,11 @@ __global__ void __launch_bounds__(W * 32, 16 / W) moe_decode_int4_kernel(const M
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k) {
                     if (u0 + k >= 2 * nc) break;
-                    rows.group(w[k], sc[k], 1.0f, (u0 + k) >> 1, lane, acc[k & 1]);
+                    row.group(w[k], sc[k], 1.0f, (u0 + k) >> 1, lane, acc[k & 1]);
                     unit(k, u0 + k + kAhead);
                 }
-            rows.finish(acc[0], lane, total[0]);
-            rows.finish(acc[1], lane, total[NM - 1]);
+            row.finish(acc[0], total[0]);
+            row.finish(acc[1], total[NM - 1]);
         }
     } else {
         // the token's experts side by side: a group's expert changes every G groups
@@ -151,17 +151,17 @@ __global__ void __launch_bounds__(W * 32, 16 / W) moe_decode_int4_kernel(const M
             auto valid = [&](int s) { return (unsigned)p.ids[s] < (unsigned)p.E; };
             bool all_valid = true;
             for (int s = s0; s <= s1; ++s) all_valid &= valid(s);
-            if (all_valid) rows.stage(a, 0, nc, lane);
-            else rows.stage(a, 0, nc, lane, [&](int i) { return valid(z * p.topk + (at + i) / G); });
+            if (all_valid) row.stage(a, nc, lane);
+            else row.stage(a, nc, lane, [&](int i) { return valid(z * p.topk + (at + i) / G); });
             float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
             for (int u0 = 0; u0 < nc; u0 += kAhead)
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k) {
                     if (u0 + k >= nc) break;
-                    rows.group(w[k], sc[k], factor[k], u0 + k, lane, acc);
+                    row.group(w[k], sc[k], factor[k], u0 + k, lane, acc);
                     unit(k, u0 + k + kAhead);
                 }
-            rows.finish(acc, lane, total[0]);
+            row.finish(acc, total[0]);
         }
     }
     if ((lane & 3) == 0) {
