@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(W * 32, kResident / W) gemv_int4_kernel(const 
 
 template <int W, class DT, int POSTOP, bool OUT_F32>
 __global__ void __launch_bounds__(W * 32, kResident / W)
-    gemv_int4_digit_kernel(const gemv::Params p, int pbytes) {
+    gemv_int4_digit_kernel(const gemv::Params p, int most) {  // most: groups of any warp
     extern __shared__ __align__(128) char smem[];  // [W][32][8] partial sums, then the warps' planes
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2;
@@ -88,9 +88,7 @@ __global__ void __launch_bounds__(W * 32, kResident / W)
         st.load();
     }
     pdl_wait();  // the weights are on their way; the activations are the previous kernel's
-    int4::DigitRow<DT> row;
-    row.pbytes = pbytes;
-    row.planes = smem + W * 1024 + warp * 3 * pbytes;
+    int4::DigitRow<DT> row(smem + W * 1024 + warp * int4::DigitRow<DT>::bytes(most), most);
     row.stage(p.A + (size_t)g0 * kGS, ng, lane);
     float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
     for (int i = 0; i < ng; ++i) {
@@ -185,12 +183,11 @@ template <int W, class DT, int POSTOP, bool OUT_F32>
 cudaError_t launch_digit(const GemvArgs &a, int most) {
     const gemv::Params p = gemv::gemv_params_impl(a);
     auto kern = gemv_int4_digit_kernel<W, DT, POSTOP, OUT_F32>;
-    const int pbytes = int4::plane_bytes(most);
-    const size_t smem = (size_t)W * (1024 + 3 * pbytes);
+    const size_t smem = (size_t)W * (1024 + int4::DigitRow<DT>::bytes(most));
     const cudaError_t e = ensure_smem(kern, smem);
     if (e != cudaSuccess) return e;
     return launch_kernel_cluster(kern, dim3((a.N + 31) / 32, a.SK), dim3(W * 32), smem, a.stream,
-                                 dim3(1, a.cluster ? a.SK : 1, 1), p, pbytes);
+                                 dim3(1, a.cluster ? a.SK : 1, 1), p, most);
 }
 
 template <int W, class DT, int POSTOP, bool OUT_F32>

@@ -12,13 +12,14 @@
 // For one row there is an integer form with a third of the instructions: a word is two
 // A registers of mma.sync m16n8k32 s8 x s8 (its even and odd rows as 16 * code, three
 // operations for eight weights), against digit planes of the activations.  With 2^e such that
-// |A| * 2^e < 2^22 (digit_common.cuh), i = round(A * 2^e) is split into three balanced base-256
+// |A| * 2^e < 2^22 in a group, i = round(A * 2^e) is split into three balanced base-256
 // digits, i = d0 + 256 d1 + 65536 d2 with d in [-128, 127]: adding 0x808080 makes them the bytes
 // of a positive number, and flipping each top bit makes those bytes signed.  The planes are
 // the first three of the MMA's eight n-columns; a group's dots (|sum 16 code d| <=
-// 128 * 128 * 128 = 2^21) are exact and read as floats from the accumulator's start pattern.
-// Elements more than 2^11 below the largest of the row's range lose bits beyond fp16's, at
-// most 2^-22 of that largest.  (5120x248320 at M = 1: 130 us against 150 us in 16 bits.)
+// 128 * 128 * 128 = 2^21) are exact, read as floats from the accumulator's start pattern and
+// scaled by 2^-e and S.  Elements more than 2^11 below the largest of their group lose bits beyond
+// fp16's, at most 2^-22 of that largest; groups do not touch each other.
+// (5120x248320 at M = 1: 121 us against 147 us in 16 bits.)
 #pragma once
 #include "common.cuh"
 #include "digit_common.cuh"
@@ -120,13 +121,6 @@ __device__ __forceinline__ void imma(int32_t (&d)[4], uint32_t a0, uint32_t a1, 
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 2^-e / 16 (the weights are 16 x code); NaN when the maximum is Inf or NaN
-template <class DT>
-__device__ __forceinline__ float inverse_scale(uint32_t mx_bits, int e) {
-    const bool bad = DT::kBF16 ? mx_bits >= 0x7F80u : mx_bits >= 0x7C00u;
-    return bad ? __int_as_float(0x7FC00000) : __int_as_float((127 - e - 4) << 23);
-}
-
 // max |value| of 8 packed activations, as magnitude bits
 __device__ __forceinline__ uint32_t absmax_bits(const uint4 v) {
     uint32_t mx = __vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu);
@@ -164,43 +158,53 @@ __device__ __forceinline__ void word_digits(const uint4 v, int e, uint2 (&out)[3
 template <class DT>
 struct DigitRow {
     char *planes;
-    int pbytes;  // of a plane
-    float rs;    // what an integer of the planes counts
+    int pbytes;   // of a plane
+    float *step;  // [kStage] of the warp: what an integer of a group's planes counts / 16 (the weights are 16 x code)
 
-    // `use(group)`: false has that group's activations taken as zeros
-    template <class Use>
-    __device__ __forceinline__ void stage(const uint16_t *a0, int ng, int lane, Use use) {
-        __syncwarp();  // the planes' last readers are through
+    // shared memory of a warp whose stages have `groups` groups at most
+    __host__ __device__ static constexpr int bytes(int groups) { return 3 * plane_bytes(groups) + kStage * 4; }
+    __device__ __forceinline__ DigitRow(char *mem, int groups) {
+        pbytes = plane_bytes(groups);
+        planes = mem;
+        step = reinterpret_cast<float *>(mem + 3 * pbytes);
+    }
+
+    // half a warp per group, a lane 8 activations of it
+    __device__ __forceinline__ void stage(const uint16_t *a0, int ng, int lane) {
         const uint4 *a = reinterpret_cast<const uint4 *>(a0);
-        uint32_t mx = 0;
+        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+        uint4 next = lane < 16 * ng ? __ldg(a + lane) : zero;
+        __syncwarp();  // the planes' last readers are through
 #pragma unroll 1
-        for (int u = lane; u < 16 * ng; u += 32)
-            if (use(u >> 4)) mx = max(mx, absmax_bits(__ldg(a + u)));
-        mx = __reduce_max_sync(0xffffffffu, mx);
-        const int e = digit::exponent_for<DT>(mx);
-        rs = inverse_scale<DT>(mx, e);
-#pragma unroll 1
-        for (int u = lane; u < 16 * ng; u += 32) {  // word row u
+        for (int u = lane; u - lane < 16 * ng; u += 32) {  // word row u
+            const uint4 v = next;
+            next = u + 32 < 16 * ng ? __ldg(a + u + 32) : zero;
+            uint32_t mx = absmax_bits(v);
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            const float top = DT::tof((uint16_t)mx);
+            // top < 2^(E - 126), E the exponent's bits
+            const int e = min(22 + 126 - (int)(__float_as_uint(top) >> 23), 120);
             uint2 d[3];
-            word_digits<DT>(use(u >> 4) ? __ldg(a + u) : make_uint4(0u, 0u, 0u, 0u), e, d);
+            word_digits<DT>(v, e, d);
+            if (u >= 16 * ng) continue;
             char *dst = planes + (u / 16) * 128 + (u & 3) * 32 + ((u >> 2) & 3) * 8;
 #pragma unroll
             for (int k = 0; k < 3; ++k) *reinterpret_cast<uint2 *>(dst + k * pbytes) = d[k];
+            // (an Inf or a NaN makes the group's sums NaN)
+            if ((u & 15) == 0) step[u / 16] = top < INFINITY ? __int_as_float((127 - e - 4) << 23) : NAN;
         }
         __syncwarp();
     }
 
-    __device__ __forceinline__ void stage(const uint16_t *a0, int ng, int lane) {
-        stage(a0, ng, lane, [](int) { return true; });
-    }
-
     // acc += (staged group i) x w, scaled by s4 * factor: acc[b][c] is column 4g + 2b + (c >> 1),
-    // plane 2t + (c & 1)
+    // plane 2t + (c & 1).  `there` false: w and s4 are zeros, whatever the group holds.
     __device__ __forceinline__ void group(const uint4 (&w)[4], const uint2 s4, float factor, int i, int lane,
-                                          float (&acc)[2][4]) const {
+                                          float (&acc)[2][4], bool there = true) const {
         const int g = lane >> 2, t = lane & 3;
         const char *b0 = planes + (g < 3 ? g : 0) * pbytes + t * 32 + i * 128;
         const uint32_t mask = g < 3 ? 0xffffffffu : 0u;
+        const float f = there ? step[i] : 0.0f, zero = -digit::kMagic * f;
         int32_t d[2][4];
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -223,7 +227,7 @@ struct DigitRow {
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-                acc[b][c] = fmaf(__int_as_float(d[b][c]) - digit::kMagic, s[2 * b + (c >> 1)], acc[b][c]);
+                acc[b][c] = fmaf(fmaf(__int_as_float(d[b][c]), f, zero), s[2 * b + (c >> 1)], acc[b][c]);
     }
 
     // total[j] += acc's planes at column 4g + j, in the lanes with t = 0
@@ -233,8 +237,7 @@ struct DigitRow {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const float next = __shfl_down_sync(0xffffffffu, acc[b][2 * c], 1);  // plane 2
-                const float r = (acc[b][2 * c] + 256.0f * acc[b][2 * c + 1]) + 65536.0f * next;
-                total[2 * b + c] = fmaf(r, rs, total[2 * b + c]);
+                total[2 * b + c] += (acc[b][2 * c] + 256.0f * acc[b][2 * c + 1]) + 65536.0f * next;
             }
     }
 };

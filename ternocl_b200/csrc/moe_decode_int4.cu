@@ -58,9 +58,8 @@ __global__ void __launch_bounds__(W * 32, 16 / W) moe_decode_int4_kernel(const M
     const int G = p.K / kGS;
     const int all = MODE == kGateUp ? G : p.topk * G;
     const int g0 = (int)((long long)all * warp / W), ng = (int)((long long)all * (warp + 1) / W) - g0;
-    int4::DigitRow<DT> row;
-    row.pbytes = int4::plane_bytes((all + W - 1) / W);
-    row.planes = smem + warp * 3 * row.pbytes;
+    const int most = (all + W - 1) / W;  // groups of any warp
+    int4::DigitRow<DT> row(smem + warp * int4::DigitRow<DT>::bytes(most), most);
 
     pdl_wait();  // ids and activations come from the kernels before
 
@@ -74,6 +73,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) moe_decode_int4_kernel(const M
     uint4 w[kAhead][4];
     uint2 sc[kAhead];
     float factor[kAhead];
+    bool there[kAhead];
     bool bad_id = false;
     auto expert = [&](int slot) {
         const int e = p.ids[slot];
@@ -133,6 +133,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) moe_decode_int4_kernel(const M
                     f = DT::tof(p.RW[slot]);
                 }
                 factor[k] = f;
+                there[k] = e >= 0;
                 if (e >= 0) {
                     load(k, 0, e, lg);
                 } else {  // contributes zero
@@ -145,20 +146,13 @@ __global__ void __launch_bounds__(W * 32, 16 / W) moe_decode_int4_kernel(const M
             };
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) unit(k, k);
-            // a left-out expert's activations must not reach the others through the planes' common scale
-            const uint16_t *a = a0 + (size_t)c0 * kGS;
-            const int at = g0 + c0, s0 = z * p.topk + at / G, s1 = z * p.topk + (at + nc - 1) / G;
-            auto valid = [&](int s) { return (unsigned)p.ids[s] < (unsigned)p.E; };
-            bool all_valid = true;
-            for (int s = s0; s <= s1; ++s) all_valid &= valid(s);
-            if (all_valid) row.stage(a, nc, lane);
-            else row.stage(a, nc, lane, [&](int i) { return valid(z * p.topk + (at + i) / G); });
+            row.stage(a0 + (size_t)c0 * kGS, nc, lane);
             float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
             for (int u0 = 0; u0 < nc; u0 += kAhead)
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k) {
                     if (u0 + k >= nc) break;
-                    row.group(w[k], sc[k], factor[k], u0 + k, lane, acc);
+                    row.group(w[k], sc[k], factor[k], u0 + k, lane, acc, there[k]);
                     unit(k, u0 + k + kAhead);
                 }
             row.finish(acc, total[0]);
@@ -188,7 +182,7 @@ template <int W, int MODE, class DT>
 cudaError_t launch_w(const MParams &p, int rows, cudaStream_t st) {
     auto kern = moe_decode_int4_kernel<W, MODE, DT>;
     const int all = (MODE == kGateUp ? 1 : p.topk) * (p.K / kGS);
-    const size_t smem = (size_t)W * 3 * int4::plane_bytes((all + W - 1) / W);  // <= 50 KB
+    const size_t smem = (size_t)W * int4::DigitRow<DT>::bytes((all + W - 1) / W);  // <= 51 KB
     const cudaError_t e = ensure_smem(kern, smem);
     if (e != cudaSuccess) return e;
     return launch_kernel(kern, dim3((unsigned)p.strips * (unsigned)rows), dim3(W * 32), smem, st, p);

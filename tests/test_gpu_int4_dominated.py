@@ -42,3 +42,26 @@ def test_linear(cuda, tl, bf16, large, M, K, N):
     check(C, *product64(A, matrix64(B, S), False), "large %g" % large)
     rows = A.abs().amax(1, keepdim=True) == A.abs()
     assert bool((codes64(B)[rows.any(0)] == 0).any()) and tl.device_error() == 0
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("weight", [0.0, 2.0 ** -14])
+@pytest.mark.parametrize("T,topk,K", [(64, 8, 128), (1, 5, 768), (64, 8, 768), (1, 3, 4096)])
+def test_down_sum_of_one_expert_with_a_large_row(cuda, tl, bf16, weight, T, topk, K):
+    """A token's rows of H each in values of one size, the first's 2^20 times the others' and weighing (almost)
+    nothing: the others' products keep their bits."""
+    g, dt, E, N = gen(T * K), DT[bf16], 5, 144
+    H = torch.randint(1, 128, (T * topk, K), generator=g, device="cuda").double()
+    H *= torch.where(torch.rand(H.shape, generator=g, device="cuda") < 0.5, 1.0, -1.0) * 2.0 ** -14
+    H[::topk] *= 2.0 ** 20
+    H = H.to(dt)
+    ids = torch.randint(0, E, (T * topk,), generator=g, device="cuda", dtype=torch.int32)
+    RW = torch.rand(T * topk, generator=g, device="cuda").to(dt)
+    RW[::topk] = weight
+    B, S = weights(g, E, K, N, dtype=dt)
+    O = tl.moe_decode_down_sum_int4(ids, H, RW, B, S, E, topk)
+    for t in range(T):
+        rows = range(t * topk, (t + 1) * topk)
+        W = torch.cat([matrix64(B[ids[r]], S[ids[r]]) * RW[r].double() for r in rows])
+        check(O[t][None], *product64(H[list(rows)].reshape(1, -1), W, False), "token %d" % t)
+    assert tl.device_error() == 0
