@@ -358,9 +358,7 @@ int ternocl_moe_decode_down_sum(const int32_t *ids, const void *H, const void *R
  *
  * Linear layer:  C[m,n] = DT(epi( sum_k A[m,k] * code(B[k,n]) * S[k/128, n] )).
  * algo: GEMV (decode, in blocks of 8 rows), GEMM (from 9 rows on: tcgen05, or for up to 24 rows
- * and many columns warp-level MMAs), or AUTO (the GEMV up to M = 8).  With M = 1 the GEMV takes
- * the activations of a row as fixed-point numbers, off by at most 2^-22 of the largest of
- * their 128-row group (2^-121, if that is more), and a row with an Inf or a NaN gives NaN.  No workspace:
+ * and many columns warp-level MMAs), or AUTO (the GEMV up to M = 8).  No workspace:
  * a K split stays within one thread-block cluster.  M <= 524280; C and Other 16-byte aligned. */
 int ternocl_int4_upcvt(const void *A, const uint32_t *B, const void *S, void *C, const void *Other,
                        const void *Bias, int M, int N, int K, int dtype, int postop, int out_f32, int algo,
@@ -377,7 +375,6 @@ int ternocl_moe_gemm_int4(const int32_t *meta, const void *A_all, const uint32_t
 /* MoE decode with 4-bit experts, as ternocl_moe_decode_gate_up and _down_sum: every routed
  * (token, expert) pair in one launch; B* [E, K/8, N], S* [E, K/128, N].  An expert id outside
  * [0, E) contributes zero, whatever its rows hold, and sets bit 1 of ternocl_device_error.
- * Activations are taken as ternocl_int4_upcvt's at M = 1.
  *   gate_up:   H[g, n] = DT(silu(X[g/topk] . gate_e[:, n]) * (X[g/topk] . up_e[:, n]))
  *   down_sum:  O[t, n] = DT(sum_j RW[g] * (H[g] . down_e[:, n])),  g = t*topk + j, e = ids[g] */
 int ternocl_moe_decode_gate_up_int4(const int32_t *ids, const void *X, const uint32_t *Bg, const void *Sg,

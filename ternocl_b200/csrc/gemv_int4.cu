@@ -85,17 +85,23 @@ __global__ void __launch_bounds__(W * 32, kResident / W)
     st.width(p.N);
     if (ng > 0) {
         st.seek(p.B, p.S, p.N, g0, n0, lane);
-        st.load();
+        st.prefetch();
     }
     pdl_wait();  // the weights are on their way; the activations are the previous kernel's
     int4::DigitRow<DT> row(smem + W * 1024 + warp * int4::DigitRow<DT>::bytes(most), most);
     row.stage(p.A + (size_t)g0 * kGS, ng, lane);
+    if (ng > 0) st.load();
     float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
     for (int i = 0; i < ng; ++i) {
         const uint4 w[4] = {st.w[0], st.w[1], st.w[2], st.w[3]};
         const uint2 s4 = st.s;
         if (i + 1 < ng) st.load();
         row.group(w, s4, 1.0f, i, lane, acc);
+    }
+    for (unsigned left = row.left(); left; left &= left - 1) {
+        const int grp = g0 + (__ffs(left) - 1) / 2;
+        st.seek(p.B, p.S, p.N, grp, n0, lane);
+        row.left_out(st, p.A + (size_t)grp * kGS, 1.0f, lane, acc);
     }
     pdl_launch_dependents();
     float total[4] = {0.f, 0.f, 0.f, 0.f};

@@ -12,14 +12,15 @@
 // For one row there is an integer form with a third of the instructions: a word is two
 // A registers of mma.sync m16n8k32 s8 x s8 (its even and odd rows as 16 * code, three
 // operations for eight weights), against digit planes of the activations.  With 2^e such that
-// |A| * 2^e < 2^22 in a group, i = round(A * 2^e) is split into three balanced base-256
-// digits, i = d0 + 256 d1 + 65536 d2 with d in [-128, 127]: adding 0x808080 makes them the bytes
-// of a positive number, and flipping each top bit makes those bytes signed.  The planes are
-// the first three of the MMA's eight n-columns; a group's dots (|sum 16 code d| <=
+// |A| * 2^e < 2^30 in a group, i = A * 2^e is split into four balanced base-256 digits,
+// i = d0 + 256 d1 + 65536 d2 + 2^24 d3 with d in [-128, 127]: adding 0x80808080 makes them the bytes
+// of an unsigned number, and flipping each top bit makes those bytes signed.  The planes are
+// the first four of the MMA's eight n-columns; a group's dots (|sum 16 code d| <=
 // 128 * 128 * 128 = 2^21) are exact, read as floats from the accumulator's start pattern and
-// scaled by 2^-e and S.  Elements more than 2^11 below the largest of their group lose bits beyond
-// fp16's, at most 2^-22 of that largest; groups do not touch each other.
-// (5120x248320 at M = 1: 121 us against 147 us in 16 bits.)
+// scaled by 2^-e and S in fp32.  Every i is exact: a group whose exponents are too far apart for
+// that (bf16: more than 2^22, fp16: 2^19) or that holds an Inf or a NaN is multiplied in 16 bits
+// after the others, its words read again.  That is 1 group in 10,000 of normal values, 1 in
+// 1,000 of products of them in bf16.  (5120x248320 at M = 1: 125 us against 147 us in 16 bits.)
 #pragma once
 #include "common.cuh"
 #include "digit_common.cuh"
@@ -46,6 +47,12 @@ struct WordStream {
         const int col = n0 + 4 * (lane >> 2) < N ? n0 + 4 * (lane >> 2) : 0;
         wp = B + ((size_t)grp * kWordsPerGroup + (lane & 3)) * N + col;
         sp = S + (size_t)grp * N + col;
+    }
+    // the next group's words into L2.  Loads into registers before the digits are staged would share
+    // scoreboards with the activations' and hold them up: 14336x4096 12.1 us, so 11.1.
+    __device__ __forceinline__ void prefetch() const {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(wp + c * row4));
     }
     // (one load in a loop, whatever moved the pointers: a second one in a branch of its own kept
     // the compiler from overlapping it with the arithmetic)
@@ -106,6 +113,7 @@ __device__ __forceinline__ void multiply(WordStream &st, const uint16_t *arow, b
 
 // ---- the integer form ------------------------------------------------------------------
 constexpr int kStage = 16;  // groups whose digit planes a warp holds
+constexpr int kPlanes = 4;
 // bytes of a plane: 128 per group; the 16 more put the planes of two neighbouring lanes' rows
 // on the two 16-byte halves of every 32 bytes (conflict-free 16-byte reads)
 __host__ __device__ constexpr int plane_bytes(int groups) { return (groups < kStage ? groups : kStage) * 128 + 16; }
@@ -121,27 +129,30 @@ __device__ __forceinline__ void imma(int32_t (&d)[4], uint32_t a0, uint32_t a1, 
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// max |value| of 8 packed activations, as magnitude bits
-__device__ __forceinline__ uint32_t absmax_bits(const uint4 v) {
-    uint32_t mx = __vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu);
-    mx = __vmaxu2(mx, __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
-    return max(mx & 0xFFFFu, mx >> 16);
+// of 8 packed activations: max |value| in the high half, 0xFFFF - (min non-zero |value| - 1) in
+// the low half (0 if there is none), as magnitude bits
+__device__ __forceinline__ uint32_t extent(const uint4 v) {
+    const uint32_t m[4] = {v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu, v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu};
+    const uint32_t mx = __vmaxu2(__vmaxu2(m[0], m[1]), __vmaxu2(m[2], m[3]));
+    uint32_t mn = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)  // 0x8000 - magnitude, 0x8000 itself for 0 -> 0
+        mn = __vmaxu2(mn, (0x80008000u - m[k]) & 0x7FFF7FFFu);
+    return (max(mx & 0xFFFFu, mx >> 16) << 16) | max(mn & 0xFFFFu, mn >> 16);
 }
 
 // the 8 activations of a word (v: packed pairs, rows in order) -> per digit plane d its even
 // and its odd rows' bytes, out[d] = (rows 0,2,4,6 | rows 1,3,5,7)
 template <class DT>
-__device__ __forceinline__ void word_digits(const uint4 v, int e, uint2 (&out)[3]) {
-    const float up = __int_as_float((127 + e) << 23);  // 2^e
+__device__ __forceinline__ void word_digits(const uint4 v, float up, uint2 (&out)[4]) {
     const uint32_t h2[4] = {v.x, v.y, v.z, v.w};
     uint32_t x[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
         const uint16_t h = (uint16_t)((k & 1) ? h2[k / 2] >> 16 : h2[k / 2] & 0xFFFFu);
-        // bits of 1.5 * 2^23 + i -> i + 0x808080
-        x[k] = __float_as_uint(fmaf(DT::tof(h), up, digit::kMagic)) + (0x00808080u - digit::kMagicBits);
+        x[k] = (uint32_t)__float2int_rn(DT::tof(h) * up) + 0x80808080u;
     }
-    uint32_t r[2][3];
+    uint32_t r[2][4];
 #pragma unroll
     for (int o = 0; o < 2; ++o) {
         const uint32_t p01 = __byte_perm(x[o], x[o + 2], 0x5140), p23 = __byte_perm(x[o + 4], x[o + 6], 0x5140);
@@ -149,9 +160,10 @@ __device__ __forceinline__ void word_digits(const uint4 v, int e, uint2 (&out)[3
         r[o][0] = __byte_perm(p01, p23, 0x5410) ^ 0x80808080u;
         r[o][1] = __byte_perm(p01, p23, 0x7632) ^ 0x80808080u;
         r[o][2] = __byte_perm(q01, q23, 0x5410) ^ 0x80808080u;
+        r[o][3] = __byte_perm(q01, q23, 0x7632) ^ 0x80808080u;
     }
 #pragma unroll
-    for (int d = 0; d < 3; ++d) out[d] = make_uint2(r[0][d], r[1][d]);
+    for (int d = 0; d < 4; ++d) out[d] = make_uint2(r[0][d], r[1][d]);
 }
 
 // An activation row of up to kStage groups as digit planes in the warp's shared memory.
@@ -159,52 +171,68 @@ template <class DT>
 struct DigitRow {
     char *planes;
     int pbytes;   // of a plane
-    float *step;  // [kStage] of the warp: what an integer of a group's planes counts / 16 (the weights are 16 x code)
+    float *step;  // [kStage]: 2^-e / 16 (the weights are 16 x code) of every group, 0 of those left out; then left()
 
     // shared memory of a warp whose stages have `groups` groups at most
-    __host__ __device__ static constexpr int bytes(int groups) { return 3 * plane_bytes(groups) + kStage * 4; }
+    __host__ __device__ static constexpr int bytes(int groups) { return kPlanes * plane_bytes(groups) + kStage * 4 + 16; }
     __device__ __forceinline__ DigitRow(char *mem, int groups) {
         pbytes = plane_bytes(groups);
         planes = mem;
-        step = reinterpret_cast<float *>(mem + 3 * pbytes);
+        step = reinterpret_cast<float *>(mem + kPlanes * pbytes);
     }
 
-    // half a warp per group, a lane 8 activations of it
+    // Two passes over the activations, whose exponents meet in between (in the planes' memory): all loads of a pass
+    // are on their way together.
     __device__ __forceinline__ void stage(const uint16_t *a0, int ng, int lane) {
+        constexpr int kMant = DT::kBF16 ? 7 : 10, kBias = DT::kBF16 ? 127 : 15;
         const uint4 *a = reinterpret_cast<const uint4 *>(a0);
-        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-        uint4 next = lane < 16 * ng ? __ldg(a + lane) : zero;
+        uint32_t *ext = reinterpret_cast<uint32_t *>(planes);
         __syncwarp();  // the planes' last readers are through
+#pragma unroll 2
+        for (int u = lane; u < 16 * ng; u += 32) ext[u] = extent(__ldg(a + u));  // word row u
+        __syncwarp();
+        // two lanes per group
+        uint32_t r = 0;
+        if (lane < 2 * ng) {
+            const uint4 x = reinterpret_cast<const uint4 *>(ext)[2 * lane], y = reinterpret_cast<const uint4 *>(ext)[2 * lane + 1];
+            r = __vmaxu2(__vmaxu2(__vmaxu2(x.x, x.y), __vmaxu2(x.z, x.w)), __vmaxu2(__vmaxu2(y.x, y.y), __vmaxu2(y.z, y.w)));
+        }
+        r = __vmaxu2(r, __shfl_xor_sync(0xffffffffu, r, 1));
+        // exponents of the largest and the smallest value (a subnormal has the lowest one's)
+        const int mx = (int)(r >> 16), mn = 0x8000 - (int)(r & 0xFFFFu);
+        const int top = max(mx >> kMant, 1), low = max(mn >> kMant, 1);
+        const int e = 29 + kBias - top;  // |value| < 2^(top - kBias + 1)
+        // the last bit of the smallest counts 1 or more; 2^e and 2^-e / 16 are normal fp32
+        const bool exact = top - low <= 29 - kMant && top < (DT::kBF16 ? 255 : 31) && e <= 122;
+        const unsigned out = __ballot_sync(0xffffffffu, !exact && mx != 0) & 0x55555555u;
+        if ((lane & 1) == 0 && lane < 2 * ng) step[lane / 2] = exact && mx != 0 ? __int_as_float((123 - e) << 23) : 0.0f;
+        if (lane == 0) step[kStage] = __uint_as_float(out);
+        __syncwarp();
 #pragma unroll 1
-        for (int u = lane; u - lane < 16 * ng; u += 32) {  // word row u
-            const uint4 v = next;
-            next = u + 32 < 16 * ng ? __ldg(a + u + 32) : zero;
-            uint32_t mx = absmax_bits(v);
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            const float top = DT::tof((uint16_t)mx);
-            // top < 2^(E - 126), E the exponent's bits
-            const int e = min(22 + 126 - (int)(__float_as_uint(top) >> 23), 120);
-            uint2 d[3];
-            word_digits<DT>(v, e, d);
-            if (u >= 16 * ng) continue;
+        for (int u = lane; u < 16 * ng; u += 32) {
+            const int s = __float_as_int(step[u / 16]);  // 2^e has the exponent 250 - that of 2^(-4 - e)
+            uint2 d[kPlanes];
+            word_digits<DT>(__ldg(a + u), s ? __int_as_float((250 << 23) - s) : 0.0f, d);
             char *dst = planes + (u / 16) * 128 + (u & 3) * 32 + ((u >> 2) & 3) * 8;
 #pragma unroll
-            for (int k = 0; k < 3; ++k) *reinterpret_cast<uint2 *>(dst + k * pbytes) = d[k];
-            // (an Inf or a NaN makes the group's sums NaN)
-            if ((u & 15) == 0) step[u / 16] = top < INFINITY ? __int_as_float((127 - e - 4) << 23) : NAN;
+            for (int k = 0; k < kPlanes; ++k) *reinterpret_cast<uint2 *>(dst + k * pbytes) = d[k];
         }
         __syncwarp();
     }
+    // the groups that stage() left out: bit 2i for group i.  (Kept in shared memory: the loops over the
+    // groups have no register for it.)
+    __device__ __forceinline__ unsigned left() const {
+        return __float_as_uint(*reinterpret_cast<volatile float *>(step + kStage));
+    }
 
     // acc += (staged group i) x w, scaled by s4 * factor: acc[b][c] is column 4g + 2b + (c >> 1),
-    // plane 2t + (c & 1).  `there` false: w and s4 are zeros, whatever the group holds.
+    // plane 2t + (c & 1)
     __device__ __forceinline__ void group(const uint4 (&w)[4], const uint2 s4, float factor, int i, int lane,
-                                          float (&acc)[2][4], bool there = true) const {
+                                          float (&acc)[2][4]) const {
         const int g = lane >> 2, t = lane & 3;
-        const char *b0 = planes + (g < 3 ? g : 0) * pbytes + t * 32 + i * 128;
-        const uint32_t mask = g < 3 ? 0xffffffffu : 0u;
-        const float f = there ? step[i] : 0.0f, zero = -digit::kMagic * f;
+        const char *b0 = planes + (g < kPlanes ? g : 0) * pbytes + t * 32 + i * 128;
+        const uint32_t mask = g < kPlanes ? 0xffffffffu : 0u;
+        const float f = step[i], zero = -digit::kMagic * f;
         int32_t d[2][4];
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -230,14 +258,22 @@ struct DigitRow {
                 acc[b][c] = fmaf(fmaf(__int_as_float(d[b][c]), f, zero), s[2 * b + (c >> 1)], acc[b][c]);
     }
 
+    // acc += factor * (a group that stage() left out) in 16 bits, as plane 0: `st` at that group,
+    // `a` its activations
+    __device__ __forceinline__ static void left_out(WordStream &st, const uint16_t *a, float factor, int lane,
+                                                    float (&acc)[2][4]) {
+        st.load();
+        multiply<DT>(st, a + 8 * (lane & 3), lane < 4, 1, factor, acc);
+    }
+
     // total[j] += acc's planes at column 4g + j, in the lanes with t = 0
-    __device__ __forceinline__ void finish(const float (&acc)[2][4], float (&total)[4]) const {
+    __device__ __forceinline__ static void finish(const float (&acc)[2][4], float (&total)[4]) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const float next = __shfl_down_sync(0xffffffffu, acc[b][2 * c], 1);  // plane 2
-                total[2 * b + c] += (acc[b][2 * c] + 256.0f * acc[b][2 * c + 1]) + 65536.0f * next;
+                const float r = acc[b][2 * c] + 256.0f * acc[b][2 * c + 1];  // planes 0, 1 here and 2, 3 at t = 1
+                total[2 * b + c] += r + 65536.0f * __shfl_down_sync(0xffffffffu, r, 1);
             }
     }
 };

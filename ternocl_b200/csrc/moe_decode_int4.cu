@@ -73,7 +73,6 @@ __global__ void __launch_bounds__(W * 32, 16 / W) moe_decode_int4_kernel(const M
     uint4 w[kAhead][4];
     uint2 sc[kAhead];
     float factor[kAhead];
-    bool there[kAhead];
     bool bad_id = false;
     auto expert = [&](int slot) {
         const int e = p.ids[slot];
@@ -90,6 +89,12 @@ __global__ void __launch_bounds__(W * 32, 16 / W) moe_decode_int4_kernel(const M
         for (int c = 0; c < 4; ++c) w[k][c] = ldg_stream128(wp + c * row4);
         sc[k] = ldg_stream64((m ? p.S1 : p.S0) + grp * p.N + col);
     };
+    int4::WordStream st;  // to prefetch, and of the groups that the digits leave out
+    st.width(p.N);
+    auto prefetch = [&](int m, int e, int lg) {
+        st.seek(m ? p.B1 : p.B0, m ? p.S1 : p.S0, p.N, e * G + lg, n0, lane);
+        st.prefetch();
+    };
     if constexpr (MODE == kGateUp) {
         const int e = expert(z);
         for (int c0 = 0; c0 < ng && e >= 0; c0 += int4::kStage) {
@@ -98,9 +103,11 @@ __global__ void __launch_bounds__(W * 32, 16 / W) moe_decode_int4_kernel(const M
             auto unit = [&](int k, int u) {
                 if (u < 2 * nc) load(k, k & 1, e, g0 + c0 + (u >> 1));
             };
+            prefetch(0, e, g0 + c0);
+            prefetch(1, e, g0 + c0);
+            row.stage(a0 + (size_t)c0 * kGS, nc, lane);
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) unit(k, k);
-            row.stage(a0 + (size_t)c0 * kGS, nc, lane);
             float acc[2][2][4];
 #pragma unroll
             for (int m = 0; m < 2; ++m)
@@ -115,6 +122,15 @@ __global__ void __launch_bounds__(W * 32, 16 / W) moe_decode_int4_kernel(const M
                     row.group(w[k], sc[k], 1.0f, (u0 + k) >> 1, lane, acc[k & 1]);
                     unit(k, u0 + k + kAhead);
                 }
+            for (unsigned left = row.left(); left; left &= left - 1) {
+                const int i = c0 + (__ffs(left) - 1) / 2;
+#pragma unroll 1
+                for (int m = 0; m < 2; ++m) {
+                    st.seek(m ? p.B1 : p.B0, m ? p.S1 : p.S0, p.N, e * G + g0 + i, n0, lane);
+                    if (m) row.left_out(st, a0 + (size_t)i * kGS, 1.0f, lane, acc[1]);
+                    else row.left_out(st, a0 + (size_t)i * kGS, 1.0f, lane, acc[0]);
+                }
+            }
             row.finish(acc[0], total[0]);
             row.finish(acc[1], total[NM - 1]);
         }
@@ -133,7 +149,6 @@ __global__ void __launch_bounds__(W * 32, 16 / W) moe_decode_int4_kernel(const M
                     f = DT::tof(p.RW[slot]);
                 }
                 factor[k] = f;
-                there[k] = e >= 0;
                 if (e >= 0) {
                     load(k, 0, e, lg);
                 } else {  // contributes zero
@@ -144,17 +159,24 @@ __global__ void __launch_bounds__(W * 32, 16 / W) moe_decode_int4_kernel(const M
                 }
                 ++lg;
             };
+            if (e >= 0 && lg < G) prefetch(0, e, lg);  // (the next chunk may start at an expert's end)
+            row.stage(a0 + (size_t)c0 * kGS, nc, lane);
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) unit(k, k);
-            row.stage(a0 + (size_t)c0 * kGS, nc, lane);
             float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
             for (int u0 = 0; u0 < nc; u0 += kAhead)
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k) {
                     if (u0 + k >= nc) break;
-                    row.group(w[k], sc[k], factor[k], u0 + k, lane, acc, there[k]);
+                    row.group(w[k], sc[k], factor[k], u0 + k, lane, acc);
                     unit(k, u0 + k + kAhead);
                 }
+            for (unsigned left = row.left(); left; left &= left - 1) {
+                const int i = c0 + (__ffs(left) - 1) / 2, at = z * p.topk + (g0 + i) / G, e1 = p.ids[at];
+                if (e1 < 0 || e1 >= p.E) continue;
+                st.seek(p.B0, p.S0, p.N, e1 * G + (g0 + i) % G, n0, lane);
+                row.left_out(st, a0 + (size_t)i * kGS, DT::tof(p.RW[at]), lane, acc);
+            }
             row.finish(acc, total[0]);
         }
     }
@@ -182,7 +204,7 @@ template <int W, int MODE, class DT>
 cudaError_t launch_w(const MParams &p, int rows, cudaStream_t st) {
     auto kern = moe_decode_int4_kernel<W, MODE, DT>;
     const int all = (MODE == kGateUp ? 1 : p.topk) * (p.K / kGS);
-    const size_t smem = (size_t)W * int4::DigitRow<DT>::bytes((all + W - 1) / W);  // <= 51 KB
+    const size_t smem = (size_t)W * int4::DigitRow<DT>::bytes((all + W - 1) / W);  // <= 67 KB
     const cudaError_t e = ensure_smem(kern, smem);
     if (e != cudaSuccess) return e;
     return launch_kernel(kern, dim3((unsigned)p.strips * (unsigned)rows), dim3(W * 32), smem, st, p);
