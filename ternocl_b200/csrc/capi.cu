@@ -207,11 +207,11 @@ static GemvPlan gemv_i8_plan(int M, int N, int K, bool allow_ws) {
 // int4 GEMV (gemv_int4.cu): 32 columns x 8 rows per CTA; an SM holds 3 CTAs of 8 warps or 7 of 4;
 // split-K within a cluster.  Measured from CUDA graphs (bf16, us, 8 warps / 4 warps per CTA):
 //  - K is split while the strips leave SMs without a CTA and every warp keeps 4 groups:
-//    14336x4096 M=1 one CTA per strip 14.7, two 10.9; 4096x4096 4.4 and 5.0;
+//    14336x4096 M=1 one CTA per strip 15.7, two 11.2, M=8 16.9 and 12.1; 4096x4096 M=1 4.3 and 5.1;
 //  - 4 warps where their rounds of 7 CTAs per SM, counted in strips, are below 1.2 times the
-//    rounds of 3 of 8 warps: 4096x28672 (6.05 strips per SM) M=1 17.3 / 14.7, M=8 19.5 / 17.3;
-//    5376x21504 M=1 17.1 / 15.3, M=8 19.0 / 16.6; 5120x65536 39.5 / 33.4 and 42.7 / 39.9;
-//    5120x248320 136 / 122 and 160 / 148; but 5120x34816 (7.35) M=1 23.3 / 25.0.
+//    rounds of 3 of 8 warps: 4096x28672 (6.05 strips per SM) M=1 17.1 / 14.2, M=2 19.4 / 17.9, M=8 19.7 /
+//    17.4; 5376x21504 M=1 16.8 / 15.2, M=8 19.6 / 16.9; 5120x65536 40.9 / 34.9 and 42.9 / 40.1;
+//    5120x248320 144 / 128 and 165 / 153; but 5120x34816 (7.35) M=1 23.4 / 24.9, M=8 25.2 / 28.9.
 static GemvPlan gemv_i4_plan(int M, int N, int K) {
     const int G = K / kGS, sms = sm_count();
     const long long tiles = (long long)((N + 31) / 32) * ((M + 7) / 8);

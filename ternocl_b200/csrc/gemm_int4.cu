@@ -36,9 +36,11 @@
 // decode takes ~1000 cycles from its words' arrival to the MMA, so NT teams keep NT steps in
 // flight, every stage has one barrier that says "filled" and one that says "free", and the
 // MMA issuer waits once per step.  Measured on B200 (bf16, CUDA graph): 14336x4096 M=2047 with
-// a residual 175-190 us = 1260-1380 TFLOP/s (floor 140 us at the burst peak), 4096x4096 M=2048
-// 57 us, 4096x4096 M=64 11.9 us; grouped 32768 rows x 768 x 2048 over 128 experts with SwiGLU
-// 175 us (floor 60).
+// a residual 193-204 us in runs of some ms, 222 us = 1080 TFLOP/s over a second of load (1605 MHz under
+// the power cap; floor 140 us at the burst peak), 4096x4096 M=2048 56-62 us; few rows 5376x21504 M=32 33.6 us
+// (9.5), M=64 40.9 (9.8), M=128 48.9 (17.2), M=512 112 (69); 4096x4096 M=64 12.0, M=512 24.3 (10.0); grouped
+// 32768 rows x 768 x 2048 over 128 experts with SwiGLU 175 us (floor 60), 12.5 rows per expert 53, 24 62,
+// 48 72 us (17.5, 18.8, 21.5).
 // Every mbarrier wait is bounded (tc::mbar_wait); on a timeout the roles stop, the producers
 // wait (bounded) for their copies in flight, and TMEM is freed.
 #include <cuda.h>

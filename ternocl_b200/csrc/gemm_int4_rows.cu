@@ -12,9 +12,12 @@
 // shared memory, so that stores and the other CTAs' shares (distributed shared memory, in split
 // order) are whole rows.
 //
-// Bound by issue: ~180 instructions decode a group of 32 columns, ~55 more per block of 8 rows.
-// Measured on B200 (bf16, CUDA graph): 5376x21504 M=9 22.7 us, M=16 23.5 us (on the tcgen05 GEMM
-// 31.0 and 31.6), M=24 28.5 us (33.0); floor 9.4 us, the words once.
+// ~180 instructions decode a group of 32 columns, ~55 more multiply a block of 8 rows.  No unit is full: on
+// 5376x64512 at M = 24 L1's data pipe is at 55 %, the tensor pipe at 40 %, DRAM at 29 %, and an instruction
+// issues in 47 % of the cycles; the 4 warps per scheduler that 128 registers leave wait for the
+// tensor pipe (a third of their stalls), for fixed latencies and at the group's barrier.
+// Measured on B200 (bf16, CUDA graph): 5376x21504 M=9 22.7-26.8 us, M=16 23.5-24.2 us (on the tcgen05 GEMM
+// 31.0 and 31.6), M=24 28.7 us (33.0); floor 9.4 us, the words once.
 #include <cuda_runtime.h>
 
 #include "common.cuh"

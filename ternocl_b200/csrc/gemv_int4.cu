@@ -7,25 +7,26 @@
 // gemv::finish, in a fixed order.
 //
 // M = 1: the same on the integer form, for ranges of up to kStage groups per warp.  (With the digits
-// of two rows it was slower than the 16-bit form: 4096x28672 M=2 21.1 against 18.6 us, 4096x4096
-// 5.5 / 5.1, 14336x4096 12.8 / 11.9, 5120x34816 25.9 / 24.9, 5120x248320 148.9 / 147.7.)
+// of two rows it was slower than the 16-bit form: 4096x28672 M=2 21.1 against 18-20 us, 4096x4096
+// 5.5 / 5.1, 14336x4096 12.8 / 11.9, 5120x34816 25.9 / 25.2, 5120x248320 149 / 145-149.)
 //
 // Grouped by expert, with 8 rows per expert or fewer on average: the M >= 2 form on the rows of one
 // expert in blocks of 8.
 //
-// Bound by HBM, with issue close behind (the 16-bit form needs 314 instructions per group and
-// warp, the integer one ~110).  Weights go straight to registers: no ring in shared memory
+// What bounds it: L1's data pipe is the busiest unit (76 % of the time at M = 1, 79 % at M = 8 on
+// 5120x124160, where DRAM is at 60 and 53 % of its peak and an instruction issues in 54 and 63 % of the
+// cycles); a group of a warp takes 236 instructions at M = 1 (the product ~110, the rest staging and
+// a CTA's ends) and 297 at M = 8.  Weights go straight to registers: no ring in shared memory
 // leaves 24 to 28 resident warps per SM with 2 KB each in flight, and a warp nothing to wait for
 // before its first words (on the cp.async ring of gemv_common.cuh 5120x248320 at M = 2 took
 // 223 us, 2.9 TB/s).  Reading further ahead (2 to 4 groups at 80 to 128 registers) measured
 // the same or slower, and so did CTAs that walk several strips with the planes kept and the
 // next strip's words on their way (134 against 130 us).
-// Measured on B200 (bf16, CUDA graph, us; floor = words and scales at 6.45 TB/s): 4096x4096 M=1 4.45
-// (1.3), M=8 5.65; 4096x28672 M=1 14.7 (9.4), M=8 17.3; 5376x21504 M=1 15.3 (9.3), M=8 16.6;
-// 14336x4096 M=1 10.9 (4.7); 5120x248320 M=1 122 (102), M=2 147, M=8 148.  ncu, 5120x124160 M=1:
-// DRAM reads = words + scales, issue 54 % busy, 256 instructions per group and warp with a CTA's
-// ends counted in.  Grouped, 536 rows x 2048 x 768 over 128 experts 28.5 us (floor 16.4; 46 us on
-// the tcgen05 kernel, whose tiles would hold 4 rows), 128 rows 18.0.
+// Measured on B200 (bf16, CUDA graph, us; floor = words and scales at 6.45 TB/s): 4096x4096 M=1 4.3
+// (1.3), M=8 5.0-5.3; 4096x28672 M=1 14.1 (9.4), M=8 17.4; 5376x21504 M=1 15.3 (9.3), M=8 16.8;
+// 14336x4096 M=1 11.2 (4.7), M=8 12.1; 5120x248320 M=1 121-129 (102), M=2 145-149, M=8 148-155.
+// Grouped, 536 rows x 2048 x 768 over 128 experts 28.6 us (floor 16.4; 46 us on the tcgen05 kernel,
+// whose tiles would hold 4 rows), 128 rows 18.2 (10.5).
 #include <cuda_runtime.h>
 
 #include "gemv_common.cuh"
@@ -219,9 +220,10 @@ cudaError_t int4_gemv_launch(const GemvArgs &a) {
     });
 }
 
-// 4 warps split K, or 2 where that left a warp fewer than 4 groups: 536 rows over 128 experts, K 2048,
-// 768 columns 28.8 us with 4 and 28.1 with 2, and 128 rows 18.9 and 21.5; K 768, 2048 columns 40.7 and 30.9
-// (24 resident warps).
+// 4 warps split K, or 2 where that left a warp fewer than 4 groups.  With 4 and with 2 warps, 128 experts,
+// us: K 768 (2048 columns) 536 rows 37.8 / 29.2, 128 rows 22.1 / 19.1; K 1024 (1024) 536 rows 22.9 / 21.1; K 1536
+// (1024) 29.4 / 29.0 and 18.6 / 19.7; K 2048 (768) 28.3 / 27.9 and 17.9 / 21.4; K 4096 (768) 50.6 / 50.8 and
+// 31.8 / 41.1.
 cudaError_t int4_gemv_grouped_launch(const GemvArgs &a, const int *meta, int E) {
     const GroupedParams p{meta, (const uint16_t *)a.A, a.B, (const uint16_t *)a.S, a.C, (const uint16_t *)a.Other,
                           a.M, a.N, a.K, E};

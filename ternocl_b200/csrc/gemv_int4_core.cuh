@@ -20,7 +20,8 @@
 // scaled by 2^-e and S in fp32.  Every i is exact: a group whose exponents are too far apart for
 // that (bf16: more than 2^22, fp16: 2^19) or that holds an Inf or a NaN is multiplied in 16 bits
 // after the others, its words read again.  That is 1 group in 10,000 of normal values, 1 in
-// 1,000 of products of them in bf16.  (5120x248320 at M = 1: 125 us against 147 us in 16 bits.)
+// 1,000 of products of them in bf16.  (At M = 1 in the integer form, at M = 2 in 16 bits:
+// 4096x28672 14.2 and 18.1 us, 5120x248320 129 and 147.)
 #pragma once
 #include "common.cuh"
 #include "digit_common.cuh"
@@ -49,7 +50,7 @@ struct WordStream {
         sp = S + (size_t)grp * N + col;
     }
     // the next group's words into L2.  Loads into registers before the digits are staged would share
-    // scoreboards with the activations' and hold them up: 14336x4096 12.1 us, so 11.1.
+    // scoreboards with the activations' and hold them up: 14336x4096 11.5 us, so 11.1.
     __device__ __forceinline__ void prefetch() const {
 #pragma unroll
         for (int c = 0; c < 4; ++c) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(wp + c * row4));

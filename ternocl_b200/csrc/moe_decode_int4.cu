@@ -13,10 +13,12 @@
 //
 // An expert id outside [0, E) contributes zero, whatever its activations, and sets bit 1 of the device error word.
 //
-// Bound by latency for one token (ids, then words, then one or two groups per warp) and by the
-// many short CTAs for several.  Measured on B200 (K 2048, N 768 and back, 128 experts, top-8, CUDA
-// graph): gate_up 1 token 6.0 us (floor 2.0: every touched expert's words once), 9 tokens 25.4 us
-// (14.2); down_sum 6.0 us (1.0) and 15.4 us (7.1).
+// Bound by latency for one token (ids, then words, then one or two groups per warp).  For several no unit is
+// full: at 9 tokens L1's data pipe is at 56 % (down_sum 45 %), DRAM at 38 % (28 %), and the 4 warps per
+// scheduler that 128 registers leave wait for loads most of the time; tokens that share an expert read
+// its words again, from L2.  Measured on B200 (K 2048, N 768 and back, 128 experts, top-8, CUDA
+// graph): gate_up 1 token 6.2-6.7 us (floor 2.0: every touched expert's words once), 9 tokens 25.2 us
+// (14.2); down_sum 6.3-6.6 us (1.0) and 15.1 us (7.1).
 #include <cuda_runtime.h>
 
 #include "common.cuh"
@@ -211,8 +213,8 @@ cudaError_t launch_w(const MParams &p, int rows, cudaStream_t st) {
 }
 
 // 8 warps split K while the CTAs fill the SMs less than twice, else 4, whose longer ranges spend
-// less on their ends: gate_up (K 2048, N 768, top-8) 1 token 5.9 against 7.3 us, 2 tokens 10.2
-// against 9.1, 9 tokens 29.4 against 25.4; down_sum 4 tokens 9.1 against 11.7, 9 tokens 16.4
+// less on their ends: gate_up (K 2048, N 768, top-8) 1 token 6.2 against 7.3 us, 2 tokens 10.1
+// against 8.6, 9 tokens 31.2 against 25.3; down_sum 4 tokens 8.9 against 11.6, 9 tokens 16.9
 // against 15.4.
 template <int MODE>
 cudaError_t launch(const MParams &p, int rows, int sms, int dtype, cudaStream_t st) {

@@ -18,7 +18,8 @@
 // Else the choice is first made on fp32 scores, one expert past topk, and stands if every gap
 // between neighbours exceeds what fp32 can be off by; a token that fails the test (1 in 100
 // or fewer on random logits, and exact ties) is done again in 64 bits, and so is one that
-// chooses a score below 2^-100.
+// chooses a score below 2^-100.  The weights of the other tokens are made in fp32 too, within 2^-20 of
+// themselves: less than half a step of the 16-bit types, a few units in the last place of fp32.
 //
 // A segment of 32 or 16 lanes per token: lane l holds experts IPL l .. IPL l + IPL - 1, so that
 // a group is a few neighbouring lanes.  A value becomes an unsigned key that orders as the value
@@ -26,11 +27,13 @@
 // steps is a local maximum, the segment's maximum, and the lowest lane that holds it.
 //
 // Bound by latency (topk dependent steps) for few tokens, where a warp per token reduces with one
-// instruction, and by issue for many: that instruction (REDUX) takes an SM ~19 cycles, so
-// there two tokens share a warp and reduce with shuffles.
+// instruction.  For many it is the steps' arithmetic and their dependences: an instruction issues in 60 %
+// of the cycles (57 % with groups), the ALU pipe is busy for 50 %, DRAM for 4 %.  That one instruction
+// (REDUX) takes an SM ~19 cycles, so there two tokens share a warp and reduce with shuffles.
 // Measured on B200 (GPU time in a CUDA graph): 16381 tokens of 128 bf16 logits, softmax, top-8
 // 11.7 us (0.78 us of HBM time), 1 token 2.8 us; sigmoid with a bias, 8 of 256 experts in 4 of 8
-// groups: 1 token 5.3 us, 16384 tokens 39.7 us.
+// groups: 1 token 5.3 us, 16384 tokens 40-42 us (2.7); groups that are not a power of two of whole lanes,
+// 64 bits throughout: 6 of 160 experts in 3 of 8 groups, 1 token 8.6 us, 16384 tokens 71 us (1.7).
 #include <cuda_runtime.h>
 #include <float.h>
 #include <math.h>
