@@ -399,7 +399,7 @@ int ternocl_moe_decode_down_sum_int4(const int32_t *ids, const void *H, const vo
  * (lowest index first), weight 0; a group with fewer than group_top unmasked experts comes
  * after the others.  A logit of +inf counts as the largest finite fp32.  Where the sum is 0 in 64
  * bits the weights are 0.  So ids always holds topk distinct experts of [0, E).  A weight is off by at most
- * 2^-20 of itself before it is rounded to RW's type.
+ * 2^-19 of itself before it is rounded to RW's type.
  * logits [T, E] and RW [T, topk] in their own types (fp16, bf16 or fp32).  E <= 1024,
  * T <= 2^30, topk <= 32 and <= topk_group * E / n_group, n_group <= 32 dividing E. */
 typedef enum { TERNOCL_SCORE_SOFTMAX = 0, TERNOCL_SCORE_SIGMOID = 1 } ternocl_score;

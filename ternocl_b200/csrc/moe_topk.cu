@@ -18,8 +18,8 @@
 // Else the choice is first made on fp32 scores, one expert past topk, and stands if every gap
 // between neighbours exceeds what fp32 can be off by; a token that fails the test (1 in 100
 // or fewer on random logits, and exact ties) is done again in 64 bits, and so is one that
-// chooses a score below 2^-100.  The weights of the other tokens are made in fp32 too, within 2^-20 of
-// themselves: less than half a step of the 16-bit types, a few units in the last place of fp32.
+// chooses a score below 2^-100.  The weights of the other tokens are made in fp32 too, within 2^-19 of
+// themselves by the bound below: far less than half a step of the 16-bit types.
 //
 // A segment of 32 or 16 lanes per token: lane l holds experts IPL l .. IPL l + IPL - 1, so that
 // a group is a few neighbouring lanes.  A value becomes an unsigned key that orders as the value
