@@ -127,3 +127,23 @@ def test_ternary_layer(cuda, tl, int8):
     want = run(X, stand_in, RW0, B, S, B, S, D, Sd, E + 1, topk, int8)
     assert torch.equal(got, want) and bool(got.any()) and not bool(got[-1].any())
     assert tl.device_error() == 0
+
+
+@pytest.mark.parametrize("T", [2, 150, 2000])
+def test_layers_without_any_row(cuda, tl, T):
+    """Every id left out: zeros from each layer, whatever the unused rows hold."""
+    import ternocl_b200.torch_ops  # noqa: F401
+    g = gen(T)
+    E, topk, H, I = 4, 2, 256, 128
+    X = torch.full((T, H), float("nan"), device="cuda").half()
+    ids = torch.full((T, topk), -1, dtype=torch.int32, device="cuda")
+    RW = torch.ones(T, topk, device="cuda").half()
+    up, down = weights(g, E, H, I, dtype=torch.float16), weights(g, E, I, H, dtype=torch.float16)
+    ops = torch.ops.ternocl
+    for O in (ops.moe_prefill_int4(X, ids, RW, *up, *up, *down, E, topk),
+              ops.moe_decode_int4(X, ids, RW, *up, *up, *down, E, topk)):
+        assert bool((O == 0).all())
+    up2, down2 = (up[0][:, ::2].contiguous(), up[1]), (down[0][:, ::2].contiguous(), down[1])
+    for int8 in (False, True):
+        assert bool((ops.moe_prefill(X, ids, RW, *up2, *up2, *down2, E, topk, int8) == 0).all())
+    assert tl.device_error(reset=True) == 2
